@@ -1,0 +1,417 @@
+"""The operators behind training a sequence decoder past teacher forcing, as cases that can be timed and checked.
+
+Three families, each with its plain form (elementary torch operations in 32 bits) and its 64-bit value:
+
+- the gated linear recurrence h_t = (1 - z_t) n_t + z_t h_{t-1}, z = sigmoid(gz), n = tanh(gn), over a whole
+  sequence with its gradient, and for one token;
+- the probability of given tokens under a row of logits, and the two losses made of it: the clipped policy loss
+  with a KL term, and the preference loss of paired sequences, each with its gradient;
+- dropout whose mask is a function of (seed, step, stream, place) and is made again in the backward pass.
+"""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+_DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+_SIZE = {"bf16": 2, "fp16": 2, "fp32": 4}
+
+
+def listed():
+    return [
+        # one token for each of 8 images x 10 beams, hidden size of the decoder: latency alone
+        dict(name="step_beam", op="step", b=80, d=256, dtype="bf16"),
+        # the decoder's training batch at its longest caption, padded
+        dict(name="scan_decoder", op="scan", b=16, t=200, d=256, dtype="bf16", train=True, masked=True, carried=True),
+        # one very long sequence read into a state, no gradient, odd sizes
+        dict(name="scan_prefill", op="scan", b=1, t=50001, d=1000, dtype="fp32", train=False, masked=False, carried=False),
+        # a large training batch of long sequences
+        dict(name="scan_long", op="scan", b=8, t=8192, d=2048, dtype="bf16", train=True, masked=False, carried=True),
+        # scores of beam hypotheses with the 112-token dictionary
+        dict(name="logprob_beam", op="logprob", b=80, t=64, k=112, dtype="fp32"),
+        # a frozen reference scoring a batch over a large vocabulary
+        dict(name="logprob_large", op="logprob", b=8, t=512, k=131072, dtype="bf16"),
+        # fine-tuning on sampled captions: the training batch of the benchmark
+        dict(name="policy_decoder", op="policy", b=16, t=32, k=112, dtype="bf16", kl=0.05),
+        # the same over a large vocabulary and long samples
+        dict(name="policy_large", op="policy", b=8, t=1024, k=32768, dtype="bf16", kl=0.05),
+        # pairs of a good and a bad caption of one image
+        dict(name="preference_decoder", op="preference", b=16, t=48, k=112, dtype="fp32"),
+        # few pairs, an odd vocabulary, logits in 32 bits
+        dict(name="preference_odd", op="preference", b=6, t=701, k=50001, dtype="fp32"),
+        # what one bottleneck layer of the encoder drops, channels last
+        dict(name="dropout_encoder", op="dropout", n=16 * 32 * 128, c=24, dtype="bf16", p=0.2, residual=False),
+        # dropout before the residual sum of a wide layer
+        dict(name="dropout_residual", op="dropout", n=16384, c=4096, dtype="fp16", p=0.1, residual=True),
+    ]
+
+
+def _spread(rng, lo, hi):
+    """A size between lo and hi, even over the logarithm."""
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 1)))))))
+
+
+def draw(rng):
+    op = rng.choice(("step", "scan", "scan", "logprob", "policy", "policy", "preference", "preference", "dropout"))
+    dtype = rng.choice(("bf16", "bf16", "fp16", "fp32"))
+    if op == "step":
+        return dict(op=op, b=_spread(rng, 1, 4096), d=_spread(rng, 16, 4096), dtype=dtype)
+    if op == "scan":
+        t, d = _spread(rng, 1, 50000), _spread(rng, 16, 4096)
+        b = _spread(rng, 1, max(1, min(64, 67_000_000 // (t * d))))
+        return dict(op=op, b=b, t=t, d=d, dtype=dtype, train=rng.random() < 0.7, masked=rng.random() < 0.5, carried=rng.random() < 0.5)
+    if op == "dropout":
+        c = _spread(rng, 1, 8192)
+        n = _spread(rng, 1, max(1, 33_000_000 // c))
+        return dict(op=op, n=n, c=c, dtype=dtype, p=round(rng.uniform(0.01, 0.9), 3), residual=rng.random() < 0.5)
+    k = _spread(rng, 40, 131072)
+    rows = _spread(rng, 2, max(2, min(16384, 134_000_000 // k)))
+    b = 2 * _spread(rng, 1, max(1, min(32, rows // 2))) if op == "preference" else _spread(rng, 1, min(64, rows))
+    case = dict(op=op, b=b, t=max(1, rows // b), k=k, dtype=dtype)
+    if op == "policy":
+        case["kl"] = rng.choice((0.0, 0.05))
+    return case
+
+
+def _lengths(case):
+    """Ragged lengths: the first sequence is whole, the last about a quarter of it."""
+    b, t = case["b"], case["t"]
+    return [max(1, t - (3 * t * i) // (4 * b)) for i in range(b)]
+
+
+def _mask(case):
+    return (torch.arange(case["t"])[None] < torch.tensor(_lengths(case))[:, None]).float().cuda()
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    dt = _DT[case["dtype"]]
+    randn = lambda *s: torch.randn(*s, device="cuda", generator=gen)  # noqa: E731
+    s = {"case": case}
+    if case["op"] in ("step", "scan"):
+        b, d = case["b"], case["d"]
+        lead = (b,) if case["op"] == "step" else (b, case["t"])
+        # the gate before its sigmoid: memories from a few steps to some hundreds
+        g = randn(*lead, 2 * d)
+        g[..., :d] = g[..., :d] * 1.5 + 2.5
+        s["g"] = g.to(dt)
+        if case["op"] == "step":
+            s["h"] = torch.tanh(randn(b, d))
+            return s
+        s["h0"] = torch.tanh(randn(b, d)) if case["carried"] else None
+        s["mask"] = _mask(case) if case["masked"] else None
+        if case["train"]:
+            s["dh"], s["dlast"] = randn(*lead, d).to(dt), randn(b, d)
+            s["g"].requires_grad_()
+            if case["carried"]:
+                s["h0"].requires_grad_()
+        return s
+    if case["op"] == "dropout":
+        n, c = case["n"], case["c"]
+        s["x"] = randn(n, c).to(dt).requires_grad_()
+        s["residual"] = randn(n, c).to(dt).requires_grad_() if case["residual"] else None
+        s["dy"] = randn(n, c).to(dt)
+        # the counter's key and step, on the device as a training loop keeps them
+        s["rng"] = torch.tensor([seed * 7919 + 17, seed % 1000 + (5 << 33)], dtype=torch.int64, device="cuda")
+        s["stream"] = 3
+        return s
+    b, t, k = case["b"], case["t"], case["k"]
+    s["mask"] = _mask(case)
+    y = torch.randint(k, (b, t), device="cuda", generator=gen)
+    x = (randn(b, t, k) * 2.0).to(dt)
+    # a model that has learned something prefers the tokens it sampled
+    x.scatter_add_(2, y[..., None], (randn(b, t, 1) * 2 + 6).to(dt))
+    s["logits"], s["y"] = x, y
+    if case["op"] != "logprob":
+        near = torch.empty(b, t, device="cuda")
+        for i in range(b):
+            near[i] = torch.log_softmax(x[i].float(), -1).gather(-1, y[i, :, None])[:, 0]
+        s["ref"] = near + 0.1 * randn(b, t)
+        if case["op"] == "policy":
+            s["old"] = near + 0.15 * randn(b, t)
+            s["adv"] = randn(b, t) + 0.2
+        x.requires_grad_()
+    return s
+
+
+# ---------------------------------------------------------------- plain forms
+
+
+def _plain_recurrence(a, b):
+    """h_t = a_t h_{t-1} + b_t from h_{-1} = 0 along axis 1, in log2(T) doubling steps."""
+    step = 1
+    while step < a.shape[1]:
+        b = torch.cat([b[:, :step], a[:, step:] * b[:, :-step] + b[:, step:]], 1)
+        a = torch.cat([a[:, :step], a[:, step:] * a[:, :-step]], 1)
+        step *= 2
+    return b
+
+
+def _plain_scan(s):
+    case, d = s["case"], s["case"]["d"]
+    g = s["g"].detach().float()
+    z, zc, n = torch.sigmoid(g[..., :d]), torch.sigmoid(-g[..., :d]), torch.tanh(g[..., d:])
+    del g
+    if s["mask"] is not None:
+        live = s["mask"][..., None] > 0
+        z, zc, n = torch.where(live, z, 1.0), torch.where(live, zc, 0.0), torch.where(live, n, 0.0)
+    h0 = torch.zeros(case["b"], d, device=z.device) if s["h0"] is None else s["h0"].detach()
+    b = zc * n
+    b[:, 0] += z[:, 0] * h0
+    h = _plain_recurrence(z, b)
+    del b
+    out, last = h.to(s["g"].dtype), h[:, -1].clone()
+    if not case["train"]:
+        return out, last
+    up = s["dh"].float()
+    up[:, -1] += s["dlast"]
+    # delta_t = up_t + z_{t+1} delta_{t+1}: the same recurrence, from the end
+    after = torch.cat([z[:, 1:], torch.zeros_like(z[:, :1])], 1)
+    delta = _plain_recurrence(after.flip(1), up.flip(1)).flip(1)
+    del after, up
+    before = torch.cat([h0[:, None], h[:, :-1]], 1)
+    dz = delta * (before - n) * z * zc
+    dn = delta * zc * (1 - n * n)
+    dg = torch.cat([dz, dn], -1).to(s["g"].dtype)
+    return (out, last, dg, (z[:, 0] * delta[:, 0])) if case["carried"] else (out, last, dg)
+
+
+def _plain_step(s):
+    d, g = s["case"]["d"], s["g"].float()
+    z, zc, n = torch.sigmoid(g[:, :d]), torch.sigmoid(-g[:, :d]), torch.tanh(g[:, d:])
+    h = zc * n + z * s["h"]
+    return h.to(s["g"].dtype), h
+
+
+def _plain_logprob(logits, y):
+    """log p(y) in 64 bits (what follows compares it with borders and sums it), and p of every token."""
+    x = logits.detach().float()
+    top = x.amax(-1, keepdim=True)
+    e = torch.exp(x - top)
+    total = e.sum(-1, keepdim=True, dtype=torch.float64)
+    picked = x.gather(-1, y[..., None]).double() - top.double() - torch.log(total)
+    return picked[..., 0], e, total
+
+
+def _plain_grad(s, e, total, coef):
+    """coef_i (1[k = y_i] - p_ik), rounded once."""
+    d = e.mul_((-coef[..., None] / total).float())
+    d.scatter_add_(-1, s["y"][..., None], coef[..., None].float())
+    return d.to(s["logits"].dtype)
+
+
+def _plain_policy(s):
+    logp, e, total = _plain_logprob(s["logits"], s["y"])
+    m = s["mask"].double()
+    count = m.sum().clamp_min(1.0)
+    adv = s["adv"].double()
+    ratio = torch.exp(logp - s["old"].double())
+    free, clipped = ratio * adv, ratio.clamp(0.8, 1.2) * adv
+    gap = s["ref"].double() - logp
+    kl = torch.exp(gap) - gap - 1
+    beta = s["case"]["kl"]
+    loss = (m * (beta * kl - torch.minimum(free, clipped))).sum() / count
+    coef = m / count * (beta * (1 - torch.exp(gap)) - torch.where(free <= clipped, free, 0.0))
+    return loss.float(), (logp * m.sign()).float(), _plain_grad(s, e, total, coef)
+
+
+def _plain_preference(s):
+    logp, e, total = _plain_logprob(s["logits"], s["y"])
+    m = s["mask"].double()
+    pairs = m.shape[0] // 2
+    gain = (m * (logp - s["ref"].double())).sum(1)
+    margin = 0.1 * (gain[:pairs] - gain[pairs:])
+    loss = torch.log1p(torch.exp(-margin.abs())) + (-margin).clamp_min(0.0)
+    slope = -0.1 * torch.sigmoid(-margin) / pairs
+    coef = m * torch.cat([slope, -slope])[:, None]
+    return loss.mean().float(), margin.float(), _plain_grad(s, e, total, coef)
+
+
+_LOW = 0xFFFFFFFF
+
+
+def _plain_draws(s, count):
+    """16-bit draws 0..count-1: the counter-based generator of Salmon et al. (SC 2011), four words of 32 bits, seven rounds."""
+    groups = torch.arange((count + 7) // 8, device="cuda")
+    seed, step = s["rng"][0], s["rng"][1]
+    c0, c1 = groups & _LOW, (s["stream"] << 8) | (groups >> 32)
+    c2, c3 = (step & _LOW).expand_as(c0), ((step >> 32) & _LOW).expand_as(c0)
+    k0, k1 = seed & _LOW, (seed >> 32) & _LOW
+    for _ in range(7):
+        p, q = c0 * 0xD2511F53, c2 * 0xCD9E8D57
+        c0, c1, c2, c3 = ((q >> 32) & _LOW) ^ c1 ^ k0, q & _LOW, ((p >> 32) & _LOW) ^ c3 ^ k1, p & _LOW
+        k0, k1 = (k0 + 0x9E3779B9) & _LOW, (k1 + 0xBB67AE85) & _LOW
+    words = torch.stack([c0, c1, c2, c3], -1)
+    return torch.stack([words & 0xFFFF, words >> 16], -1).reshape(-1)[:count]
+
+
+def _plain_dropout(s):
+    x, p = s["x"].detach(), s["case"]["p"]
+    limit = math.floor(p * 65536 + 0.5)
+    keep = (_plain_draws(s, x.numel()) >= limit).view(x.shape)
+    scale = 65536 / (65536 - limit)
+    y = torch.where(keep, x.float() * scale, 0.0)
+    dx = torch.where(keep, s["dy"].float() * scale, 0.0).to(x.dtype)
+    if s["residual"] is None:
+        return y.to(x.dtype), dx
+    return (y + s["residual"].detach().float()).to(x.dtype), dx, s["dy"]
+
+
+# ---------------------------------------------------------------- one pass
+
+
+def run(s):
+    case = s["case"]
+    op = case["op"]
+    if not own:
+        if op == "logprob":
+            return (_plain_logprob(s["logits"], s["y"])[0] * s["mask"]).float()
+        return {"step": _plain_step, "scan": _plain_scan, "policy": _plain_policy, "preference": _plain_preference, "dropout": _plain_dropout}[op](s)
+    from wap_amd import ops
+    if op == "step":
+        return ops.gated_step(s["g"], s["h"])
+    if op == "scan":
+        if not case["train"]:
+            with torch.no_grad():
+                return ops.gated_scan(s["g"], s["h0"], s["mask"])
+        out, last = ops.gated_scan(s["g"], s["h0"], s["mask"])
+        leaves = (s["g"], s["h0"]) if case["carried"] else (s["g"],)
+        return (out, last) + torch.autograd.grad((out, last), leaves, (s["dh"], s["dlast"]))
+    if op == "logprob":
+        with torch.no_grad():
+            return ops.token_logprob(s["logits"], s["y"], s["mask"])
+    if op == "policy":
+        loss, logp = ops.policy_loss(s["logits"], s["y"], s["mask"], s["old"], s["adv"], s["ref"], kl_coef=case["kl"])
+        return loss, logp, torch.autograd.grad(loss, s["logits"])[0]
+    if op == "preference":
+        loss, margin = ops.preference_loss(s["logits"], s["y"], s["mask"], s["ref"], beta=0.1)
+        return loss, margin, torch.autograd.grad(loss, s["logits"])[0]
+    y = ops.counter_dropout(s["x"], case["p"], s["rng"], stream=s["stream"], residual=s["residual"])
+    leaves = (s["x"],) if s["residual"] is None else (s["x"], s["residual"])
+    return (y,) + torch.autograd.grad(y, leaves, s["dy"])
+
+
+# ---------------------------------------------------------------- the work and the 64-bit values
+
+
+def work(case):
+    op, w = case["op"], _SIZE[case["dtype"]]
+    if op == "step":
+        n = case["b"] * case["d"]
+        return {"bytes": n * (3 * w + 8), "flops": 12 * n}
+    if op == "scan":
+        n, live = case["b"] * case["t"] * case["d"], case["b"] * case["t"] * case["d"]
+        if case["masked"]:
+            live = sum(_lengths(case)) * case["d"]
+        rows = case["b"] * case["t"] * 4 if case["masked"] else 0
+        ends = case["b"] * case["d"] * 4
+        moved = live * 2 * w + n * w + rows + ends * (1 + case["carried"])
+        if case["train"]:
+            moved += 3 * n * w + ends * (1 + case["carried"])
+        return {"bytes": moved, "flops": live * (30 if case["train"] else 12)}
+    if op == "dropout":
+        n = case["n"] * case["c"]
+        return {"bytes": n * w * (6 if case["residual"] else 4), "flops": n * (3 if case["residual"] else 2)}
+    rows, all_rows, k = sum(_lengths(case)), case["b"] * case["t"], case["k"]
+    if op == "logprob":
+        return {"bytes": rows * k * w + all_rows * 16, "flops": 4 * rows * k}
+    # the gradient of a row that the mask leaves out is written too: zeros
+    extra = 28 if op == "policy" else 16
+    return {"bytes": (rows + all_rows) * k * w + all_rows * extra, "flops": 7 * rows * k}
+
+
+def _exact_scan(s):
+    case, d = s["case"], s["case"]["d"]
+    b, t = case["b"], case["t"]
+    if t * (2 if case["train"] else 1) > 60000 or b * t * d > 150_000_000:
+        return None
+    g = s["g"].detach()
+    live = torch.ones(b, t, 1, dtype=torch.bool, device=g.device) if s["mask"] is None else s["mask"][..., None] > 0
+    h = torch.zeros(b, d, dtype=torch.float64, device=g.device) if s["h0"] is None else s["h0"].detach().double()
+    first, hs = h, torch.empty(b, t, d, dtype=torch.float64, device=g.device)
+    for i in range(t):
+        gz, n = g[:, i, :d].double(), torch.tanh(g[:, i, d:].double())
+        h = torch.where(live[:, i], n + (h - n) / (1 + torch.exp(-gz)), h)
+        hs[:, i] = h
+    if not case["train"]:
+        return hs, h
+    dg = torch.empty(b, t, 2 * d, dtype=torch.float64, device=g.device)
+    back = s["dlast"].double()
+    for i in reversed(range(t)):
+        delta = s["dh"][:, i].double() + back
+        gz, n = g[:, i, :d].double(), torch.tanh(g[:, i, d:].double())
+        e = torch.exp(-gz)
+        past = hs[:, i - 1] if i else first
+        dg[:, i, :d] = torch.where(live[:, i], delta * (past - n) * e / (1 + e) ** 2, 0.0)
+        dg[:, i, d:] = torch.where(live[:, i], delta * (e / (1 + e)) * (1 - n * n), 0.0)
+        back = torch.where(live[:, i], delta / (1 + e), delta)
+    return (hs, h, dg, back) if case["carried"] else (hs, h, dg)
+
+
+def _exact_rows(s):
+    """log p(y), row by row of the batch."""
+    return torch.stack([torch.log_softmax(x.detach().double(), -1).gather(-1, y[:, None])[:, 0] for x, y in zip(s["logits"], s["y"])])
+
+
+def _exact_grad(s, coef):
+    d = []
+    for x, y, c in zip(s["logits"], s["y"], coef):
+        p = torch.softmax(x.detach().double(), -1) * -c[:, None]
+        p[torch.arange(y.numel(), device=y.device), y] += c
+        d.append(p)
+    return torch.stack(d)
+
+
+def _exact_dropout(s):
+    x, p = s["x"].detach(), s["case"]["p"]
+    limit, n = math.floor(p * 65536 + 0.5), x.numel()
+    seed, step = (int(v) % 2**64 for v in s["rng"].tolist())
+    low, half = np.uint64(_LOW), np.uint64(32)
+    keep = np.empty((n + 7) // 8 * 8, bool)
+    for at in range(0, (n + 7) // 8, 1 << 20):
+        group = np.arange(at, min(at + (1 << 20), (n + 7) // 8), dtype=np.uint64)
+        c = [group & low, (group >> half) | np.uint64(s["stream"] << 8), np.full_like(group, step & _LOW), np.full_like(group, step >> 32)]
+        for r in range(7):
+            k0, k1 = np.uint64((seed + r * 0x9E3779B9) & _LOW), np.uint64(((seed >> 32) + r * 0xBB67AE85) & _LOW)
+            p0, p1 = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+            c = [(p1 >> half) ^ c[1] ^ k0, p1 & low, (p0 >> half) ^ c[3] ^ k1, p0 & low]
+        u = np.stack([v >> np.uint64(16 * j) & np.uint64(0xFFFF) for v in c for j in (0, 1)], 1)
+        keep[8 * at:8 * at + u.size] = (u >= limit).reshape(-1)
+    keep = torch.from_numpy(keep[:n].reshape(tuple(x.shape))).to(x.device)
+    y = x.double() * keep / (1 - limit / 65536)
+    dx = s["dy"].double() * keep / (1 - limit / 65536)
+    return (y, dx) if s["residual"] is None else (y + s["residual"].detach().double(), dx, s["dy"].double())
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    op = case["op"]
+    if op == "scan":
+        return _exact_scan(s)
+    if op == "step":
+        gz, n = s["g"][:, :case["d"]].double(), torch.tanh(s["g"][:, case["d"]:].double())
+        h = n + (s["h"].double() - n) / (1 + torch.exp(-gz))
+        return h, h
+    if op == "dropout":
+        return _exact_dropout(s)
+    logp, m = _exact_rows(s), s["mask"].double()
+    if op == "logprob":
+        return logp * m
+    if op == "policy":
+        lr, adv, gap = logp - s["old"].double(), s["adv"].double(), s["ref"].double() - logp
+        # the clip binds where the ratio has left the range on the side that the advantage favours
+        bound = ((adv > 0) & (lr > math.log(1.2))) | ((adv < 0) & (lr < math.log(0.8)))
+        gain = torch.where(bound, torch.where(adv > 0, 1.2, 0.8).double(), lr.exp()) * adv
+        loss = (m * (case["kl"] * (torch.expm1(gap) - gap) - gain)).sum() / m.sum()
+        coef = m / m.sum() * (-case["kl"] * torch.expm1(gap) - torch.where(bound, 0.0, lr.exp() * adv))
+        return loss, logp * m, _exact_grad(s, coef)
+    half = case["b"] // 2
+    gain = ((logp - s["ref"].double()) * m).sum(1)
+    margin = 0.1 * (gain[:half] - gain[half:])
+    slope = -0.1 / half * torch.sigmoid(-margin)
+    return -torch.nn.functional.logsigmoid(margin).mean(), margin, _exact_grad(s, m * torch.cat([slope, -slope])[:, None])
