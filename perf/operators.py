@@ -168,7 +168,7 @@ def _plain_scan(s):
     out, last = h.to(s["g"].dtype), h[:, -1].clone()
     if not case["train"]:
         return out, last
-    up = s["dh"].float()
+    up = s["dh"].to(torch.float32, copy=True)
     up[:, -1] += s["dlast"]
     # delta_t = up_t + z_{t+1} delta_{t+1}: the same recurrence, from the end
     after = torch.cat([z[:, 1:], torch.zeros_like(z[:, :1])], 1)
