@@ -69,9 +69,15 @@ from .functional import (  # noqa: E402
     masked_softmax_context,
     unfold_1ch,
 )
+from .scan import gated_scan, gated_step  # noqa: E402
+from .seqloss import policy_loss, preference_loss, token_logprob  # noqa: E402
+from .dropout import counter_dropout  # noqa: E402
 
 __all__ = [
     "set_backend", "get_backend", "use_hip",
     "attention_score", "coverage_attention", "masked_softmax_context",
     "gru_cell", "gru_gates", "fused_gru_cell", "unfold_1ch",
+    "gated_scan", "gated_step",
+    "token_logprob", "policy_loss", "preference_loss",
+    "counter_dropout",
 ]
