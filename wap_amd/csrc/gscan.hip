@@ -4,8 +4,28 @@
 //   h_t = (1 - z_t) n_t + z_t h_{t-1}              masked step: h_t = h_{t-1}
 //
 // The blend is the GRU's; its gates do not see the state, so h is linear in
-// the state before and the time axis can be cut.  The state, the gates and
-// all sums are f32; h is rounded once, where it is stored.
+// the state before: a run of steps is h_out = A h_in + B, and runs compose.
+// The state, the gates and all sums are f32; h is rounded once, where it is
+// stored.
+//
+// Layout.  A workgroup takes a tile of S = W R steps by 64 VEC channels: each
+// of its W waves holds R steps in registers (one load of every gate, all of
+// them in flight together), reduces them to (A, B) and finds the state before
+// them from the waves before it (LDS) and the tiles before its own.  Tiles of
+// one channel block are chained through global memory in one launch, so that
+// gates are read once and h is written once: what a chunked scan of two
+// launches reads twice.
+//
+// The chain.  Tile c publishes (A, B) of its steps, waits until the end state
+// of one of the tiles c-1 .. c-WINDOW is there, steps over the tiles between
+// with their (A, B), and publishes its own end state.  The end state is
+// fma(A, state before, B) whichever tile the walk began at, so results do not
+// depend on timing.  Every published word shows by itself whether it has been
+// written (a pattern of ones, a NaN that no result has, stands for "not yet"),
+// so no flag has to be ordered against data; words are read and written with
+// device-scope atomics, since the eight XCDs' L2 caches are not coherent.
+// A tile waits only for tiles of earlier tickets, and a ticket is drawn by a
+// workgroup that is running already: every wait ends.
 #include <hip/hip_runtime.h>
 
 #include "opcommon.h"
@@ -14,79 +34,568 @@ namespace {
 
 using namespace wap;
 
+
 struct Gates {
-  float z, zc, n;  // z, 1 - z (from its own exponential: no cancellation), n
+  float z, zc, n;  // z, 1 - z (from the exponential: no cancellation), n
 };
 
+// 2^(x log2 e).  For 16-bit gates one multiplication and the hardware's exp2
+// (relative error |x| 2^-24) are far below the gates' own rounding; f32 gates
+// add what the product lost.
+template <typename T>
+__device__ __forceinline__ float exp_of(float x, float most) {
+  constexpr float log2e = 1.44269502162933349609375f;
+  // the smaller one, NaN if x is NaN
+  const float t = __builtin_elementwise_minimum(x * log2e, most);
+  const float e = __builtin_amdgcn_exp2f(t);
+  if constexpr (sizeof(T) == 4) {
+    // x log2 e - t, with log2 e in two parts; 0 where t is cut or infinite
+    const float lost = fmaf(x, 1.92596299112661746887e-8f, fmaf(x, log2e, -t));
+    return fabsf(t) < 120.f ? fmaf(e * 0.693147180559945309f, lost, e) : e;
+  }
+  return e;
+}
+
+// z = 1 / (1 + e), 1 - z = e z with e = exp(-gz), cut at 2^126 so that the
+// product stays finite.  tanh x = 1 - 2 / (1 + exp(2 x)), absolute error
+// 1.2e-7; near zero, where that is not enough, the odd series: to x^5 below 0.1
+// (the next term is 6e-8 of the value there), for f32 gates to x^9 below 0.3
+// (5e-8).
+template <typename T>
 __device__ __forceinline__ Gates gates(float gz, float gn) {
-  const float e = expf(-fabsf(gz));
-  const float big = 1.f / (1.f + e), small = e * big;
+  const float e = exp_of<T>(-gz, 126.f);
   Gates r;
-  r.z = gz >= 0.f ? big : small;
-  r.zc = gz >= 0.f ? small : big;
-  if (gz != gz) r.z = r.zc = gz;
-  r.n = tanhf(gn);
+  const float z = __builtin_amdgcn_rcpf(1.f + e);
+  r.zc = e * z;
+  r.z = z - 0x1p-126f;  // nothing but where e was cut: 0
+  const float f = exp_of<T>(2.f * gn, 127.f);
+  const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + f), 1.f);
+  const float q = gn * gn;
+  constexpr bool wide = sizeof(T) == 4;
+  float p = fmaf(q, 2.f / 15.f, -1.f / 3.f);
+  if constexpr (wide)
+    p = fmaf(q, fmaf(q, fmaf(q, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f),
+             -1.f / 3.f);
+  const float near = gn * fmaf(q, p, 1.f);
+  r.n = __builtin_unpredictable(fabsf(gn) < (wide ? 0.3f : 0.1f)) ? near : far;
   return r;
 }
 
-// One thread per (sequence, channel), serial over time.
-template <typename T>
-__global__ void gscan_fwd_kernel(
-    const T* __restrict__ g, long gsb, long gst, const float* __restrict__ h0,
-    const float* __restrict__ mask, T* __restrict__ out,
-    float* __restrict__ last, int B, long L, int D) {
-  const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= (long)B * D) return;
-  const long b = i / D, d = i % D;
-  float h = h0 ? h0[i] : 0.f;
-  for (long t = 0; t < L; ++t) {
-    if (!mask || mask[b * L + t] > 0.f) {
-      const T* p = g + b * gsb + t * gst + d;
-      const Gates q = gates((float)p[0], (float)p[D]);
-      h = fmaf(q.z, h, q.zc * q.n);
-    }
-    out[(b * L + t) * D + d] = (T)h;
-  }
-  last[i] = h;
+// ------------------------------------------------------------ the chain
+
+constexpr uint32_t UNSET = 0xffffffffu;
+
+struct Chain {
+  uint64_t* run;     // (A, B) of every tile's steps
+  uint32_t* end;     // end state of every tile
+  uint32_t* ticket;  // one counter a group, 128 bytes apart; null: one tile
+  int blocks;        // channel blocks of all sequences
+  int groups, per;   // blocks are dealt to groups, `per` to each at most
+  int tiles;         // tiles of one sequence
+};
+
+// A result's bits: any NaN becomes one that is not the pattern for "not yet".
+__device__ __forceinline__ uint32_t word(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return v != v ? 0x7fc00000u : u;
 }
 
-// delta_t = dh_t + z_{t+1} delta_{t+1}; the states come from a second forward
-// walk whose results wait in `hs` (f32).
-template <typename T>
-__global__ void gscan_bwd_kernel(
-    const T* __restrict__ g, long gsb, long gst, const float* __restrict__ h0,
-    const float* __restrict__ mask, const T* __restrict__ dh, long dsb,
-    long dst, const float* __restrict__ dlast, float* __restrict__ hs,
-    T* __restrict__ dg, float* __restrict__ dh0, int B, long L, int D) {
-  const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= (long)B * D) return;
-  const long b = i / D, d = i % D;
-  float h = h0 ? h0[i] : 0.f;
-  for (long t = 0; t < L; ++t) {
-    hs[(b * L + t) * D + d] = h;
-    if (!mask || mask[b * L + t] > 0.f) {
-      const T* p = g + b * gsb + t * gst + d;
-      const Gates q = gates((float)p[0], (float)p[D]);
-      h = fmaf(q.z, h, q.zc * q.n);
-    }
-  }
-  float c = dlast ? dlast[i] : 0.f;
-  for (long t = L - 1; t >= 0; --t) {
-    if (dh) c += (float)dh[b * dsb + t * dst + d];
-    T* o = dg + (b * L + t) * 2 * D + d;
-    if (mask && !(mask[b * L + t] > 0.f)) {
-      o[0] = (T)0.f;
-      o[D] = (T)0.f;
-      continue;
-    }
-    const T* p = g + b * gsb + t * gst + d;
-    const Gates q = gates((float)p[0], (float)p[D]);
-    o[0] = (T)(c * (hs[(b * L + t) * D + d] - q.n) * (q.z * q.zc));
-    o[D] = (T)(c * q.zc * (1.f - q.n * q.n));
-    c *= q.z;
-  }
-  if (dh0) dh0[i] = c;
+template <typename W>
+__device__ __forceinline__ W peek(const W* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+
+template <typename W>
+__device__ __forceinline__ void post(W* p, W v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The next tile of this workgroup's group, in time order over all channel
+// blocks of the group: (block, place in time). False: none.
+// The grid has groups * per * tiles workgroups and blockIdx % groups is the
+// group, so that with workgroups dealt to the XCDs in turn a chain stays on
+// one XCD.
+__device__ __forceinline__ bool next_tile(const Chain& ch, int* block,
+                                          int* at) {
+  const int grp = blockIdx.x % ch.groups;
+  int k = blockIdx.x / ch.groups;  // same in every lane: kept in scalars
+  if (ch.ticket) {
+    __shared__ int drawn;
+    if (threadIdx.x == 0)
+      drawn = (int)__hip_atomic_fetch_add(ch.ticket + grp * 32, 1u,
+                                          __ATOMIC_RELAXED,
+                                          __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    k = __builtin_amdgcn_readfirstlane(drawn);
+  }
+  *at = k / ch.per;
+  *block = k % ch.per * ch.groups + grp;
+  return *block < ch.blocks;
+}
+
+// What the waves of a workgroup have seen of the tiles before theirs.
+template <int VEC, int W, int EACH>
+struct Seen {
+  float end[W * EACH][64 * VEC];
+  float2 run[W * EACH][64 * VEC];
+  int has[2][W * EACH];  // 1: the end state, 2: the run; by turns
+};
+
+// A wave's place in the words of tile `at`; tiles are `stride` apart.
+template <int VEC>
+__device__ __forceinline__ long words_at(const Chain& ch, int block, int at,
+                                         int lane) {
+  return ((long)at * ch.blocks + block) * (64 * VEC) + lane * VEC;
+}
+
+// One wave publishes the run (A, B) of its tile's steps.  Nobody steps over
+// the first tile, which publishes its end state at once, or over the last.
+template <int VEC>
+__device__ __forceinline__ void publish(const Chain& ch, int block, int at,
+                                        int lane, const float (&A)[VEC],
+                                        const float (&B)[VEC]) {
+  if (at == 0 || at + 1 == ch.tiles) return;
+  uint64_t* p = ch.run + words_at<VEC>(ch, block, at, lane);
+#pragma unroll
+  for (int j = 0; j < VEC; ++j)
+    post(p + j, (uint64_t)word(A[j]) | (uint64_t)word(B[j]) << 32);
+}
+
+// The whole workgroup finds the state h before tile `at` (tile 0: h as it is)
+// and publishes the state after it; A and B count in wave 0.  Wave w looks at
+// the tiles at-1-w, at-1-w-W, ..: EACH of them, so that a workgroup steps over
+// W EACH tiles in one round trip to memory and holds few registers for it.
+template <int VEC, int W, int EACH>
+__device__ __forceinline__ void walk(const Chain& ch, int block, int at,
+                                     int wave, int lane, const float (&A)[VEC],
+                                     const float (&B)[VEC],
+                                     Seen<VEC, W, EACH>& seen,
+                                     float (&h)[VEC]) {
+  const long stride = (long)ch.blocks * (64 * VEC);  // from tile to tile
+  const long mine = words_at<VEC>(ch, block, at, lane);
+  if (at > 0) {
+    const int reach = at < W * EACH ? at : W * EACH;
+    int has[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) has[k] = 0;
+    int from = -1;  // the nearest tile before this one whose end is there
+    for (int turn = 0;; turn ^= 1) {
+      // the end first: where it is there the run is not needed, and where it
+      // is not there is time
+      uint32_t e[EACH][VEC];
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        const int i = wave + k * W;
+        if (i < reach && !(has[k] & 1)) {
+          const uint32_t* p = ch.end + mine - (i + 1) * stride;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) e[k][j] = peek(p + j);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        const int i = wave + k * W;
+        if (i < reach && !(has[k] & 1)) {
+          bool there = true;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) there &= e[k][j] != UNSET;
+          if (__all(there)) {
+            has[k] |= 1;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+              seen.end[i][lane * VEC + j] = __uint_as_float(e[k][j]);
+          } else if (i + 1 < reach && !(has[k] & 2)) {
+            // (the end of the last tile in reach is not stepped over)
+            const uint64_t* p = ch.run + mine - (i + 1) * stride;
+            uint64_t r[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) r[j] = peek(p + j);
+            there = true;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) there &= (uint32_t)r[j] != UNSET;
+            if (__all(there)) {
+              has[k] |= 2;
+#pragma unroll
+              for (int j = 0; j < VEC; ++j)
+                seen.run[i][lane * VEC + j] =
+                    make_float2(__uint_as_float((uint32_t)r[j]),
+                                __uint_as_float((uint32_t)(r[j] >> 32)));
+            }
+          }
+        }
+        if (lane == 0) seen.has[turn][i] = has[k];
+      }
+      __syncthreads();
+      // every wave comes to the same answer; the next turn writes elsewhere
+#pragma unroll
+      for (int i = W * EACH - 1; i >= 0; --i) {
+        const int q = seen.has[turn][i];
+        if (i < reach) from = q & 1 ? i : q & 2 ? from : -1;
+      }
+      from = __builtin_amdgcn_readfirstlane(from);
+      if (from >= 0) break;
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) h[j] = seen.end[from][lane * VEC + j];
+    for (int i = from - 1; i >= 0; --i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float2 q = seen.run[i][lane * VEC + j];
+        h[j] = fmaf(q.x, h[j], q.y);
+      }
+  }
+  if (wave == 0 && at + 1 < ch.tiles) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      post(ch.end + mine + j, word(fmaf(A[j], h[j], B[j])));
+  }
+}
+
+// "Not yet" everywhere, and the tickets at zero.
+__global__ void chain_clear_kernel(uint4* __restrict__ words, long n,
+                                   uint32_t* __restrict__ ticket, int m) {
+  const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < n) words[i] = make_uint4(UNSET, UNSET, UNSET, UNSET);
+  if (i < m) ticket[i] = 0u;
+}
+
+// ------------------------------------------------------------ forward
+
+struct Scan {
+  long gsb, gst;      // strides of g over sequence and time
+  long dsb, dst;      // strides of dh
+  const float* h0;    // [B, D] or null
+  const float* mask;  // [B, L] or null
+  long L;
+  int D, dblocks;     // channel blocks of one sequence
+};
+
+// The forward pass leaves the state before step MARK, 2 MARK, .. for the
+// backward pass, whose tiles begin at such steps: f32, 1 / MARK of the size of
+// h, and each pass can cut time as suits it.
+constexpr int MARK = 64;
+
+__host__ __device__ __forceinline__ long marks_of(long L) {
+  return (L - 1) / MARK;
+}
+
+// Which of this wave's steps exist and count, one bit each.
+template <int ROWS>
+__device__ __forceinline__ constexpr uint32_t all_steps() {
+  return (1u << ROWS) - 1;
+}
+
+template <int ROWS>
+__device__ __forceinline__ uint32_t steps_on(const Scan& s, long b, long t0,
+                                             int lane) {
+  bool on = lane < ROWS && t0 + lane < s.L;
+  if (on && s.mask) on = s.mask[b * s.L + t0 + lane] > 0.f;
+  return (uint32_t)__ballot(on);
+}
+
+// A lane's place in a row that is the same in all lanes: the row's address
+// stays scalar work, and the lane's 32-bit byte offset is part of the access.
+template <typename T>
+__device__ __forceinline__ T* lane_at(T* row, uint32_t bytes) {
+  typedef std::conditional_t<std::is_const_v<T>, const char, char> byte;
+  return reinterpret_cast<T*>(reinterpret_cast<byte*>(row) + bytes);
+}
+
+// Rows of a wave, kept as they came (two 16-bit values a register).  Rows past
+// the end read the last one; what is read there is not used.
+template <typename T, int VEC>
+using Pack = typename VecOf<T, VEC, sizeof(T)>::type;
+
+template <typename T, int VEC, int ROWS>
+__device__ __forceinline__ void load_rows(const T* base, uint32_t bytes,
+                                          long stride, long rows,
+                                          Pack<T, VEC> (&v)[ROWS]) {
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+    v[r] = *reinterpret_cast<const Pack<T, VEC>*>(
+        lane_at(base + (r < rows ? (long)r : rows - 1) * stride, bytes));
+}
+
+template <typename T, int VEC, int W, int ROWS>
+__global__ __launch_bounds__(64 * W) void gscan_fwd_kernel(
+    const T* __restrict__ g, Scan s, Chain ch, T* __restrict__ out,
+    float* __restrict__ last, float* __restrict__ marks) {
+  constexpr int CH = 64 * VEC;
+  constexpr int EACH = W < 8 ? 2 : 1;
+  __shared__ float2 runs[W][CH];
+  __shared__ Seen<VEC, W, EACH> seen;
+  int block, at;
+  if (!next_tile(ch, &block, &at)) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long b = block / s.dblocks;
+  const int d = block % s.dblocks * CH + lane * VEC;
+  // lanes past the last channel read its place and store nothing
+  const bool inside = d < s.D;
+  const uint32_t dc = inside ? d : s.D - VEC;
+  const uint32_t off = dc * (uint32_t)sizeof(T);
+  const long t0 = ((long)at * W + wave) * ROWS;
+  const uint32_t on = steps_on<ROWS>(s, b, t0, lane);
+  const long rows = s.L - t0;
+  float a[ROWS][VEC], x[ROWS][VEC];
+  if (on) {
+    Pack<T, VEC> rz[ROWS], rn[ROWS];
+    const T* p = g + b * s.gsb + t0 * s.gst;
+    load_rows<T, VEC, ROWS>(p, off, s.gst, rows, rz);
+    load_rows<T, VEC, ROWS>(p + s.D, off, s.gst, rows, rn);
+    // all loads leave before the first value is used
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const Gates q = gates<T>((float)rz[r][j], (float)rn[r][j]);
+        a[r][j] = q.z;
+        x[r][j] = q.zc * q.n;
+      }
+  }
+  if (on != all_steps<ROWS>()) {  // same in every lane
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (!(on >> r & 1)) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) a[r][j] = 1.f, x[r][j] = 0.f;
+      }
+  }
+  // step r becomes the run of the wave's steps up to r
+#pragma unroll
+  for (int r = 1; r < ROWS; ++r)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      x[r][j] = fmaf(a[r][j], x[r - 1][j], x[r][j]);
+      a[r][j] *= a[r - 1][j];
+    }
+  float h[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j)
+    h[j] = s.h0 ? s.h0[b * s.D + dc + j] : 0.f;
+  if (W > 1 || ch.tiles > 1) {
+    float A[VEC], B[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      A[j] = a[ROWS - 1][j], B[j] = x[ROWS - 1][j];
+      runs[wave][lane * VEC + j] = make_float2(A[j], B[j]);
+    }
+    __syncthreads();
+    if (ch.tiles > 1) {
+      if (wave == 0) {
+        for (int w = 1; w < W; ++w)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const float2 q = runs[w][lane * VEC + j];
+            A[j] *= q.x;
+            B[j] = fmaf(q.x, B[j], q.y);
+          }
+        publish<VEC>(ch, block, at, lane, A, B);
+      }
+      walk<VEC, W, EACH>(ch, block, at, wave, lane, A, B, seen, h);
+    }
+    for (int w = 0; w < wave; ++w)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float2 q = runs[w][lane * VEC + j];
+        h[j] = fmaf(q.x, h[j], q.y);
+      }
+  }
+  if (marks && t0 % MARK == 0 && t0 > 0 && inside && rows > 0) {
+    float* m = marks + (b * marks_of(s.L) + t0 / MARK - 1) * s.D + d;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) m[j] = h[j];
+  }
+  T* o = out + (b * s.L + t0) * s.D;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    T v[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = (T)fmaf(a[r][j], h[j], x[r][j]);
+    if (r < rows && inside)
+      store_vec<T, VEC>(lane_at(o + (long)r * s.D, off), v);
+  }
+  // steps past the end leave the state as it is
+  if (inside && rows > 0 && rows <= ROWS) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      last[b * s.D + d + j] = fmaf(a[ROWS - 1][j], h[j], x[ROWS - 1][j]);
+  }
+}
+
+// ------------------------------------------------------------ backward
+//
+//   delta_t = dh_t + z_{t+1} delta_{t+1}           (dlast joins the last one)
+//   dgz = delta (h_{t-1} - n) z (1 - z),  dgn = delta (1 - z) (1 - n^2)
+//
+// With c_t = z_t delta_t, the gradient that leaves step t for the state before
+// it, c_t = z_t (c_{t+1} + dh_t): the same chain, from the end.  The states
+// are made again from the states that the forward pass left, which reads less
+// than h itself would be, and has them in f32.
+
+template <typename T, int VEC, int W, int ROWS>
+__global__ __launch_bounds__(64 * W) void gscan_bwd_kernel(
+    const T* __restrict__ g, Scan s, Chain ch, const float* __restrict__ marks,
+    const T* __restrict__ dh, const float* __restrict__ dlast,
+    T* __restrict__ dg, float* __restrict__ dh0) {
+  constexpr int CH = 64 * VEC, EACH = W < 8 ? 2 : 1;
+  __shared__ float2 runs[W][CH];
+  __shared__ float back[W][CH];
+  __shared__ Seen<VEC, W, EACH> seen;
+  int block, from_end;
+  if (!next_tile(ch, &block, &from_end)) return;
+  const int at = ch.tiles - 1 - from_end;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long b = block / s.dblocks;
+  const int d = block % s.dblocks * CH + lane * VEC;
+  const bool inside = d < s.D;
+  const uint32_t dc = inside ? d : s.D - VEC;
+  const uint32_t off = dc * (uint32_t)sizeof(T);
+  const long t0 = ((long)at * W + wave) * ROWS;
+  const long rows = s.L - t0;
+  const uint32_t on = steps_on<ROWS>(s, b, t0, lane);
+  float z[ROWS][VEC], zc[ROWS][VEC], n[ROWS][VEC];
+  Pack<T, VEC> ru[ROWS];  // dh stays as it came: half the registers for 16 bits
+  if (dh && rows > 0)
+    load_rows<T, VEC, ROWS>(dh + b * s.dsb + t0 * s.dst, off, s.dst, rows, ru);
+  if (on) {
+    Pack<T, VEC> rz[ROWS], rn[ROWS];
+    const T* p = g + b * s.gsb + t0 * s.gst;
+    load_rows<T, VEC, ROWS>(p, off, s.gst, rows, rz);
+    load_rows<T, VEC, ROWS>(p + s.D, off, s.gst, rows, rn);
+    // all loads leave before the first value is used
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const Gates q = gates<T>((float)rz[r][j], (float)rn[r][j]);
+        z[r][j] = q.z;
+        zc[r][j] = q.zc;
+        n[r][j] = q.n;
+      }
+  }
+  if (on != all_steps<ROWS>()) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (!(on >> r & 1)) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) z[r][j] = 1.f, zc[r][j] = n[r][j] = 0.f;
+      }
+  }
+  if (!dh || rows < ROWS) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (!dh || r >= rows) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) ru[r][j] = (T)0.f;
+      }
+  }
+  float h[VEC], c[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    // (every wave takes its tile's first state and steps to its own)
+    h[j] = at > 0 ? marks[(b * marks_of(s.L) + (long)at * W * ROWS / MARK - 1) *
+                              s.D + dc + j]
+           : s.h0 ? s.h0[b * s.D + dc + j]
+                  : 0.f;
+    c[j] = dlast ? dlast[b * s.D + dc + j] : 0.f;
+  }
+  float A[VEC], C[VEC];
+  if (W > 1 || ch.tiles > 1) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      float B = 0.f;
+      A[j] = 1.f, C[j] = 0.f;
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        A[j] *= z[r][j];
+        B = fmaf(z[r][j], B, zc[r][j] * n[r][j]);
+      }
+#pragma unroll
+      for (int r = ROWS - 1; r >= 0; --r)
+        C[j] = z[r][j] * (C[j] + (float)ru[r][j]);
+      runs[wave][lane * VEC + j] = make_float2(A[j], B);
+      back[wave][lane * VEC + j] = C[j];
+    }
+    __syncthreads();
+    if (ch.tiles > 1) {
+      if (wave == 0) {
+        // the waves' runs from the end; this one's own is the last
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          float a = 1.f, b = 0.f;
+          for (int w = W - 1; w > 0; --w) {
+            const float q = runs[w][lane * VEC + j].x;
+            a *= q;
+            b = fmaf(q, b, back[w][lane * VEC + j]);
+          }
+          C[j] = fmaf(A[j], b, C[j]);
+          A[j] *= a;
+        }
+      }
+      if (wave == 0) publish<VEC>(ch, block, from_end, lane, A, C);
+    }
+    for (int w = 0; w < wave; ++w)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float2 q = runs[w][lane * VEC + j];
+        h[j] = fmaf(q.x, h[j], q.y);
+      }
+  }
+  // what delta is multiplied by needs the states alone: made while the chain
+  // from the end is on its way, in the place of 1 - z and n
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float past = h[j], q = zc[r][j], m = n[r][j];
+      h[j] = fmaf(z[r][j], past, q * m);
+      zc[r][j] = q * z[r][j] * (past - m);
+      n[r][j] = q * fmaf(-m, m, 1.f);
+    }
+  if (W > 1 || ch.tiles > 1) {
+    if (ch.tiles > 1)
+      walk<VEC, W, EACH>(ch, block, from_end, wave, lane, A, C, seen, c);
+    for (int w = W - 1; w > wave; --w)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        c[j] = fmaf(runs[w][lane * VEC + j].x, c[j], back[w][lane * VEC + j]);
+  }
+  T* o = dg + (b * s.L + t0) * 2 * s.D;
+#pragma unroll
+  for (int r = ROWS - 1; r >= 0; --r) {
+    float fz[VEC], fn[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float delta = c[j] + (float)ru[r][j];
+      fz[j] = delta * zc[r][j];
+      fn[j] = delta * n[r][j];
+      c[j] = z[r][j] * delta;
+    }
+    // a step that does not count has no gradient, whatever passes it by
+    if (!(on >> r & 1)) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) fz[j] = fn[j] = 0.f;
+    }
+    if (r < rows && inside) {
+      T vz[VEC], vn[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) vz[j] = (T)fz[j], vn[j] = (T)fn[j];
+      T* row = o + (long)r * 2 * s.D;
+      store_vec<T, VEC>(lane_at(row, off), vz);
+      store_vec<T, VEC>(lane_at(row + s.D, off), vn);
+    }
+  }
+  if (dh0 && inside && t0 == 0) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) dh0[b * s.D + d + j] = c[j];
+  }
+}
+
+// ------------------------------------------------------------ one token
 
 template <typename T>
 __global__ void gstep_kernel(
@@ -96,17 +605,19 @@ __global__ void gstep_kernel(
   if (i >= total) return;
   const long b = i / D, d = i % D;
   const T* p = g + b * gsb + d;
-  const Gates q = gates((float)p[0], (float)p[D]);
+  const Gates q = gates<T>((float)p[0], (float)p[D]);
   const float v = fmaf(q.z, h[i], q.zc * q.n);
   h_new[i] = v;
   out[i] = (T)v;
 }
 
+// ------------------------------------------------------------ host
+
 void check_gates(const torch::Tensor& g, int dim) {
   TORCH_CHECK(g.is_cuda(), "gated_scan: g must be on the GPU");
   TORCH_CHECK(g.dim() == dim && g.size(-1) % 2 == 0 && g.stride(-1) == 1,
               "gated_scan: g must end in a dense axis of 2 D");
-  TORCH_CHECK(g.size(-1) / 2 < (1 << 30) && g.numel() > 0,
+  TORCH_CHECK(g.size(-1) / 2 < (1 << 29) && g.numel() > 0,
               "gated_scan: empty or too wide");
 }
 
@@ -128,41 +639,172 @@ void check_mask(const c10::optional<torch::Tensor>& mask,
               "gated_scan: mask must be [B, T]");
 }
 
+// Channels of a lane, waves of a workgroup, steps of a wave.
+struct Shape {
+  int vec, waves, rows;
+};
+
+// How a pass is cut, by the number of 64-channel blocks and the length (us on
+// an MI355X; "2,8,16": two channels a lane, 8 waves of 16 steps).
+// - Up to 256 steps one tile holds the sequence, and nothing is chained: 16 x
+//   200 x 256 bf16 forward 8.2 in one tile of 1,16,16, 10.0 in two of 2,8,16.
+// - Few blocks: time is the only axis to spread over, and a round trip of the
+//   chain should step far: 1 x 40000 x 128 bf16 forward 28.7 with tiles of 256
+//   steps, 55.2 with 128; from 5 blocks on 128 (2 x 20000 x 512: 42.1, 52.1).
+// - Two channels a lane where that leaves enough workgroups, from 64 blocks:
+//   8 x 8192 x 2048 bf16 forward 194.5, with one 203.7; 8 x 4096 x 256: 21.2,
+//   19.6.  The backward pass then holds 8 steps a wave, to stay under 128
+//   registers: 321.9, with 16 steps of one channel 368.0; 8 x 4096 x 256:
+//   29.3, 27.0.
+Shape shape_of(const torch::Tensor& g, bool backward) {
+  const long L = g.size(1), D = g.size(2) / 2;
+  const long blocks = g.size(0) * ((D + 63) / 64);
+  const bool two = blocks >= 64 && D % 2 == 0 && g.element_size() == 2;
+  const int rows = L <= 8 || (backward && two) ? 8 : 16;
+  if (backward && two && L > 64 && L <= 256)  // no room for 16 steps of two
+    return {1, L <= 128 ? 8 : 16, 16};
+  if (L <= (backward && two ? 64 : 16 * rows)) {
+    int w = 1;
+    while (w * rows < L) w *= 2;
+    return {two ? 2 : 1, w, rows};
+  }
+  return {two ? 2 : 1, blocks < 5 ? 16 : 8, rows};
+}
+
+struct Cut {
+  Shape p;
+  Chain ch;
+  long words;  // published words of one kind
+  Scan s;
+};
+
+Cut cut_of(const torch::Tensor& g, const c10::optional<torch::Tensor>& h0,
+           const c10::optional<torch::Tensor>& mask, bool backward) {
+  Cut c;
+  c.s.gsb = g.stride(0);
+  c.s.gst = g.stride(1);
+  c.s.dsb = c.s.dst = 0;
+  c.s.h0 = data_or_null<float>(h0);
+  c.s.mask = data_or_null<float>(mask);
+  c.s.L = g.size(1);
+  c.s.D = g.size(2) / 2;
+  c.p = shape_of(g, backward);
+  const int wide = 64 * c.p.vec;
+  c.s.dblocks = (c.s.D + wide - 1) / wide;
+  const long blocks = (long)g.size(0) * c.s.dblocks;
+  const long step = (long)c.p.waves * c.p.rows;
+  const long tiles = (c.s.L + step - 1) / step;
+  TORCH_CHECK(blocks < (1L << 30) && tiles < (1L << 30),
+              "gated_scan: too many sequences, channels or steps");
+  c.ch.blocks = blocks;
+  c.ch.tiles = tiles;
+  c.ch.groups = tiles == 1 ? 1 : std::min(blocks, 64L);
+  c.ch.per = (blocks + c.ch.groups - 1) / c.ch.groups;
+  TORCH_CHECK((long)c.ch.groups * c.ch.per * tiles < (1L << 31),
+              "gated_scan: too many tiles");
+  c.ch.run = nullptr;
+  c.ch.end = nullptr;
+  c.ch.ticket = nullptr;
+  c.words = blocks * tiles * wide;
+  return c;
+}
+
+// Words of the chain, cleared: end states | runs | tickets.
+torch::Tensor make_chain(const torch::Tensor& g, Cut* c) {
+  const auto opts = g.options().dtype(at::kInt);
+  const long tickets = c->ch.groups * 32L;
+  auto buf = torch::empty({3 * c->words + tickets}, opts);
+  uint32_t* p = data<uint32_t>(buf);
+  c->ch.end = p;
+  c->ch.run = reinterpret_cast<uint64_t*>(p + c->words);
+  c->ch.ticket = p + 3 * c->words;
+  const long quads = 3 * c->words / 4;  // words is a multiple of 64
+  const long n = std::max(quads, tickets);
+  hipLaunchKernelGGL(chain_clear_kernel, dim3((n + 255) / 256), dim3(256), 0,
+                     stream_of(g), reinterpret_cast<uint4*>(p), quads,
+                     c->ch.ticket, (int)tickets);
+  launched("gated_scan");
+  return buf;
+}
+
+template <int VEC, int W, int ROWS>
+struct Fixed {
+  static constexpr int vec = VEC, waves = W, rows = ROWS;
+};
+
+// f(Fixed<...>) for a shape that shape_of gives.
+template <typename T, bool BACKWARD, typename F>
+void by_shape(const Shape& p, F&& f) {
+  if constexpr (sizeof(T) == 2) {
+    if (p.vec == 2) {
+      constexpr int R = BACKWARD ? 8 : 16;
+      if (p.waves == 1 && p.rows == 8) return f(Fixed<2, 1, 8>());
+      switch (p.waves) {
+        case 1: return f(Fixed<2, 1, R>());
+        case 2: return f(Fixed<2, 2, R>());
+        case 4: return f(Fixed<2, 4, R>());
+        case 8: return f(Fixed<2, 8, R>());
+      }
+      if constexpr (!BACKWARD) return f(Fixed<2, 16, R>());
+      TORCH_CHECK(false, "gated_scan: no such shape");
+    }
+  }
+  if (p.rows == 8) return f(Fixed<1, 1, 8>());
+  switch (p.waves) {
+    case 1: return f(Fixed<1, 1, 16>());
+    case 2: return f(Fixed<1, 2, 16>());
+    case 4: return f(Fixed<1, 4, 16>());
+    case 8: return f(Fixed<1, 8, 16>());
+    default: return f(Fixed<1, 16, 16>());
+  }
+}
+
 }  // namespace
 
+// -> h, last state and, with `keep` and where the backward pass takes more
+// than one tile, the states that it begins from.
 std::vector<torch::Tensor> gated_scan_fwd(
     torch::Tensor g, c10::optional<torch::Tensor> h0,
-    c10::optional<torch::Tensor> mask) {
+    c10::optional<torch::Tensor> mask, bool keep) {
   check_gates(g, 3);
   check_state(h0, g);
   check_mask(mask, g);
   c10::DeviceGuard guard(g.device());
-  const int B = g.size(0), D = g.size(2) / 2;
-  const long L = g.size(1);
+  const long B = g.size(0), L = g.size(1), D = g.size(2) / 2;
   auto out = torch::empty({B, L, D}, g.options());
   auto last = torch::empty({B, D}, g.options().dtype(at::kFloat));
-  const long blocks = ((long)B * D + 63) / 64;
+  Cut c = cut_of(g, h0, mask, false);
+  torch::Tensor buf, marks;
+  if (c.ch.tiles > 1) buf = make_chain(g, &c);
+  const Shape back = shape_of(g, true);
+  if (keep && L > (long)back.waves * back.rows)
+    marks = torch::empty({B, marks_of(L), D}, last.options());
+  const dim3 grid((long)c.ch.groups * c.ch.per * c.ch.tiles);
   by_type(g, "gated_scan", [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    hipLaunchKernelGGL(gscan_fwd_kernel<T>, dim3(blocks), dim3(64), 0,
-                       stream_of(g), data<T>(g), g.stride(0), g.stride(1),
-                       data_or_null<float>(h0), data_or_null<float>(mask),
-                       data<T>(out), data<float>(last), B, L, D);
+    by_shape<T, false>(c.p, [&](auto p) {
+      constexpr int V = decltype(p)::vec, W = decltype(p)::waves,
+                    R = decltype(p)::rows;
+      hipLaunchKernelGGL((gscan_fwd_kernel<T, V, W, R>), grid,
+                         dim3(64 * W), 0, stream_of(g), data<T>(g), c.s,
+                         c.ch, data<T>(out), data<float>(last),
+                         marks.defined() ? data<float>(marks) : nullptr);
+    });
   });
   launched("gated_scan");
+  if (marks.defined()) return {out, last, marks};
   return {out, last};
 }
 
 std::vector<torch::Tensor> gated_scan_bwd(
     torch::Tensor g, c10::optional<torch::Tensor> h0,
-    c10::optional<torch::Tensor> mask, c10::optional<torch::Tensor> dh,
-    c10::optional<torch::Tensor> dlast) {
+    c10::optional<torch::Tensor> mask, c10::optional<torch::Tensor> marks,
+    c10::optional<torch::Tensor> dh, c10::optional<torch::Tensor> dlast) {
   check_gates(g, 3);
   check_state(h0, g);
   check_state(dlast, g);
   check_mask(mask, g);
-  const int B = g.size(0), D = g.size(2) / 2;
-  const long L = g.size(1);
+  const long B = g.size(0), L = g.size(1), D = g.size(2) / 2;
   if (dh.has_value())
     TORCH_CHECK(dh->scalar_type() == g.scalar_type() &&
                     dh->device() == g.device() && dh->dim() == 3 &&
@@ -170,22 +812,41 @@ std::vector<torch::Tensor> gated_scan_bwd(
                     dh->size(2) == D && dh->stride(2) == 1,
                 "gated_scan: dh must be [B, T, D] in g's type");
   c10::DeviceGuard guard(g.device());
-  auto dg = torch::empty({B, L, 2 * (long)D}, g.options());
-  auto dh0 = torch::empty({B, D}, g.options().dtype(at::kFloat));
-  auto hs = torch::empty({B, L, D}, g.options().dtype(at::kFloat));
-  const long blocks = ((long)B * D + 63) / 64;
+  auto dg = torch::empty({B, L, 2 * D}, g.options());
+  torch::Tensor dh0;
+  if (h0.has_value()) dh0 = torch::empty_like(*h0);
+  Cut c = cut_of(g, h0, mask, true);
+  if (dh.has_value()) {
+    c.s.dsb = dh->stride(0);
+    c.s.dst = dh->stride(1);
+  }
+  torch::Tensor buf;
+  if (c.ch.tiles > 1) {
+    TORCH_CHECK(marks.has_value(), "gated_scan: the forward pass's states are "
+                                   "missing");
+    WAP_F32(*marks, g, "gated_scan");
+    TORCH_CHECK(marks->numel() == B * marks_of(L) * D &&
+                    c.p.waves * c.p.rows % MARK == 0,
+                "gated_scan: the forward pass's states are of another shape");
+    buf = make_chain(g, &c);
+  }
+  const dim3 grid((long)c.ch.groups * c.ch.per * c.ch.tiles);
   by_type(g, "gated_scan", [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    hipLaunchKernelGGL(gscan_bwd_kernel<T>, dim3(blocks), dim3(64), 0,
-                       stream_of(g), data<T>(g), g.stride(0), g.stride(1),
-                       data_or_null<float>(h0), data_or_null<float>(mask),
-                       data_or_null<T>(dh), dh.has_value() ? dh->stride(0) : 0,
-                       dh.has_value() ? dh->stride(1) : 0,
-                       data_or_null<float>(dlast), data<float>(hs),
-                       data<T>(dg), data<float>(dh0), B, L, D);
+    by_shape<T, true>(c.p, [&](auto p) {
+      constexpr int V = decltype(p)::vec, W = decltype(p)::waves,
+                    R = decltype(p)::rows;
+      hipLaunchKernelGGL((gscan_bwd_kernel<T, V, W, R>), grid,
+                         dim3(64 * W), 0, stream_of(g), data<T>(g), c.s,
+                         c.ch, data_or_null<float>(marks),
+                         data_or_null<T>(dh), data_or_null<float>(dlast),
+                         data<T>(dg),
+                         dh0.defined() ? data<float>(dh0) : nullptr);
+    });
   });
   launched("gated_scan backward");
-  return {dg, dh0};
+  if (dh0.defined()) return {dg, dh0};
+  return {dg};
 }
 
 std::vector<torch::Tensor> gated_step(torch::Tensor g, torch::Tensor h) {

@@ -926,11 +926,11 @@ torch::Tensor bnrelu_conv_fwd_mxfp8(
 // gated linear recurrence (gscan.hip)
 std::vector<torch::Tensor> gated_scan_fwd(
     torch::Tensor g, c10::optional<torch::Tensor> h0,
-    c10::optional<torch::Tensor> mask);
+    c10::optional<torch::Tensor> mask, bool keep);
 std::vector<torch::Tensor> gated_scan_bwd(
     torch::Tensor g, c10::optional<torch::Tensor> h0,
-    c10::optional<torch::Tensor> mask, c10::optional<torch::Tensor> dh,
-    c10::optional<torch::Tensor> dlast);
+    c10::optional<torch::Tensor> mask, c10::optional<torch::Tensor> marks,
+    c10::optional<torch::Tensor> dh, c10::optional<torch::Tensor> dlast);
 std::vector<torch::Tensor> gated_step(torch::Tensor g, torch::Tensor h);
 
 // token probabilities and sequence losses (seqloss.hip)

@@ -54,7 +54,9 @@ class _GatedScan(torch.autograd.Function):
         hip = _hip(g)
         if hip:
             from . import ext
-            out, last = ext.require().gated_scan_fwd(g, h0, mask)
+            out, last, *marks = ext.require().gated_scan_fwd(
+                g, h0, mask, any(ctx.needs_input_grad[:2]))
+            marks = marks[0] if marks else None
         else:
             z, zc, n = _gates(g)
             h = (torch.zeros_like(n[:, 0]) if h0 is None else h0)
@@ -65,22 +67,23 @@ class _GatedScan(torch.autograd.Function):
                     new = torch.where(mask[:, t, None] > 0, new, h)
                 h = new
                 hs.append(h)
-            out, last = torch.stack(hs, dim=1).to(g.dtype), h
+            out, last, marks = torch.stack(hs, dim=1).to(g.dtype), h, None
         ctx.hip = hip
-        ctx.save_for_backward(g, h0, mask)
+        ctx.save_for_backward(g, h0, mask, marks)
         return out, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh: Optional[Tensor], dlast: Optional[Tensor]):
-        g, h0, mask = ctx.saved_tensors
+        g, h0, mask, marks = ctx.saved_tensors
         if dh is None and dlast is None:
             return None, None, None
         if ctx.hip:
             from . import ext
             dh = None if dh is None else _dense(dh)
             dlast = None if dlast is None else dlast.contiguous()
-            dg, dh0 = ext.require().gated_scan_bwd(g, h0, mask, dh, dlast)
+            dg, *dh0 = ext.require().gated_scan_bwd(g, h0, mask, marks, dh, dlast)
+            dh0 = dh0[0] if dh0 else None
         else:
             z, zc, n = _gates(g)
             h = torch.zeros_like(n[:, 0]) if h0 is None else h0
