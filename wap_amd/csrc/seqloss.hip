@@ -36,19 +36,70 @@ __device__ __forceinline__ float weight(const Rows& r, long row) {
   return r.w ? r.w[row] : 1.f;
 }
 
-__device__ __forceinline__ long row_at(const Rows& r, long row) {
-  return row / r.T * r.sb + row % r.T * r.st;
+// Rows and sequences are below 2^31: their quotients are 32-bit work.
+__device__ __forceinline__ long row_at(const Rows& r, uint32_t row) {
+  return (long)(row / (uint32_t)r.T) * r.sb + (long)(row % (uint32_t)r.T) * r.st;
 }
 
-// Sum / max over the workgroup, on every thread. `red`: one value a wave.
+// 16 bytes of a row, which may begin at any element.
+template <typename T>
+struct Wide {
+  static constexpr int V = 16 / sizeof(T);
+  typedef typename VecOf<T, V, sizeof(T)>::type type;
+};
+
+constexpr float LOG2E = 1.44269502162933349609f;
+// log2 e = LOG2E (1 + LOST)
+constexpr double LOST = 1.92596299112661746887e-8 / 1.44269502162933349609;
+
+// log2 of exp(x - m).  x - m first: it is exact where it matters, and lowest
+// values stay finite.
+__device__ __forceinline__ float log2_from(float x, float m) {
+  return (x - m) * LOG2E;
+}
+
+__device__ __forceinline__ float exp_from(float x, float m) {
+  return __builtin_amdgcn_exp2f(log2_from(x, m));
+}
+
+// Exponentials e = 2^u of a row, added up.  What LOG2E lacks makes every e too
+// large by u LOST ln 2, always to the same side (5e-8 of the sum, and a
+// gain adds up the logarithms of hundreds): the sum of e u takes it back.
+struct Sum {
+  float s, t;
+
+  __device__ __forceinline__ void add(float x, float m) {
+    // 2^-150 is nothing beside the maximum's 1, and e u stays finite
+    const float u = __builtin_elementwise_maximum(log2_from(x, m), -150.f);
+    const float e = __builtin_amdgcn_exp2f(u);
+    s += e;
+    t = fmaf(e, u, t);
+  }
+  __device__ __forceinline__ void add(const Sum& o) {
+    s += o.s;
+    t += o.t;
+  }
+  // to another maximum, m <= top
+  __device__ __forceinline__ void move(float m, float top) {
+    const float u = __builtin_elementwise_maximum(log2_from(m, top), -150.f);
+    const float e = __builtin_amdgcn_exp2f(u);
+    t = e * fmaf(u, s, t);
+    s *= e;
+  }
+  __device__ __forceinline__ double value() const {
+    return (double)s + (double)t * (LOST * 0.693147180559945309417);
+  }
+};
+
+// Over the workgroup, on every thread; `red`: one value a wave.
+// The sum of the threads' parts is in 64 bits, for the logarithm.
 template <int NT>
-__device__ __forceinline__ float group_sum(float v, float* red) {
+__device__ __forceinline__ double group_sum(double v, double* red) {
   v = lanes_sum(v);
   if constexpr (NT == 64) return v;
-  __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  float s = 0.f;
+  double s = 0.0;
 #pragma unroll
   for (int i = 0; i < NT / 64; ++i) s += red[i];
   return s;
@@ -58,7 +109,6 @@ template <int NT>
 __device__ __forceinline__ float group_max(float v, float* red) {
   v = lanes_max(v);
   if constexpr (NT == 64) return v;
-  __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   float s = red[0];
@@ -68,16 +118,16 @@ __device__ __forceinline__ float group_max(float v, float* red) {
 }
 
 // logp of a row from its token's logit, maximum and sum.
-__device__ __forceinline__ double row_logp(float xy, float m, float sum) {
-  return (double)xy - (double)m - log((double)sum);
+__device__ __forceinline__ double row_logp(float xy, float m, double sum) {
+  return (double)xy - (double)m - log(sum);
 }
 
 // Loss of one token and its derivative by logp, both without the 1 / sum of
 // weights.  At a border of the clip the unclipped side counts.
 __device__ __forceinline__ void policy_row(
-    const Policy& p, long row, long T, double logp, double* loss,
+    const Policy& p, uint32_t row, uint32_t T, double logp, double* loss,
     double* slope) {
-  const double adv = p.adv[row / T * p.ab + row % T * p.at];
+  const double adv = p.adv[(long)(row / T) * p.ab + (long)(row % T) * p.at];
   const double ratio = exp(logp - (double)p.old_logp[row]);
   const double kept = fmin(fmax(ratio, 1.0 - p.lo), 1.0 + p.hi);
   const double free_ = adv == 0.0 ? 0.0 : ratio * adv, clipped = kept * adv;
@@ -91,100 +141,309 @@ __device__ __forceinline__ void policy_row(
   }
 }
 
-// One workgroup per row, three passes over it.  POLICY: loss and gradient in
-// the same launch.
-template <typename T, int NT, bool POLICY>
-__global__ void rows_kernel(
+// Where a row's results go.
+struct Out {
+  float* logp;       // or null
+  double* wide;      // logp in 64 bits, or null
+  float2* stats;     // maximum and sum, or null
+  double* loss;      // share of the loss (policy)
+  float *coef, *held;  // the row's c, the factor that its gradient holds
+};
+
+// A row's gradient from the values at hand: 16 bytes beginning at token k.
+template <typename T>
+__device__ __forceinline__ typename Wide<T>::type grad_of(
+    const typename Wide<T>::type& x, long k, long y, float m, float scale,
+    float c) {
+  constexpr int V = Wide<T>::V;
+  float v[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = scale * exp_from((float)x[i], m);
+  if (y >= k && y < k + V) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (k + i == y) v[i] += c;
+  }
+  typename Wide<T>::type d;
+#pragma unroll
+  for (int i = 0; i < V; ++i) d[i] = (T)v[i];
+  return d;
+}
+
+// The gradient of a row's vectors begin + lane, + step, .. below end.  What is
+// left of a row that is no multiple of V goes with the part that the next
+// vector would be in.
+template <typename T>
+__device__ __forceinline__ void grad_span(const T* x, T* d, int K, int begin,
+                                          int end, int lane, int step, long y,
+                                          float m, float scale, float c) {
+  typedef typename Wide<T>::type vec;
+  constexpr int V = Wide<T>::V;
+  const int whole = K / V;
+  for (int i = begin + lane; i < end && i < whole; i += step)
+    *reinterpret_cast<vec*>(d + (long)i * V) = grad_of<T>(
+        *reinterpret_cast<const vec*>(x + (long)i * V), (long)i * V, y, m,
+        scale, c);
+  const int k = whole * V + lane;
+  if (k < K && begin <= whole && whole < end)
+    d[k] = (T)(scale * exp_from((float)x[k], m) + (k == y ? c : 0.f));
+}
+
+template <typename T>
+__device__ __forceinline__ void zero_span(T* d, int K, int begin, int end,
+                                          int lane, int step) {
+  typedef typename Wide<T>::type vec;
+  constexpr int V = Wide<T>::V;
+  const int whole = K / V;
+  for (int i = begin + lane; i < end && i < whole; i += step) {
+    vec z;
+#pragma unroll
+    for (int j = 0; j < V; ++j) z[j] = (T)0.f;
+    *reinterpret_cast<vec*>(d + (long)i * V) = z;
+  }
+  if (whole * V + lane < K && begin <= whole && whole < end)
+    d[whole * V + lane] = (T)0.f;
+}
+
+// Rows of logits to logp, and with POLICY to the loss and, if `dlogits`, its
+// gradient, in the same launch: a row's c needs nothing but the row and the
+// sum of the weights, so logits are read once and the gradient is written
+// once, where a pass of its own would read the logits again.
+//
+// NT threads a row.  E > 0: the row waits in registers, E 16-byte vectors a
+// thread, packed as they came.  E = 0: rows too long for that are read once
+// for the sums (a running maximum and sum a thread) and again for the
+// gradient.  Bound by memory: 18 instruction slots an element of bf16 are 0.4
+// of what reading and writing it takes.
+template <typename T, int NT, int E, bool POLICY>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
     const T* __restrict__ logits, Rows r, Policy p,
-    const double* __restrict__ count, float* __restrict__ logp_out,
-    double* __restrict__ wide_out, float2* __restrict__ stats, double* __restrict__ row_loss,
-    float* __restrict__ coef, float* __restrict__ held,
-    T* __restrict__ dlogits) {
-  __shared__ float red[NT / 64];
-  const long row = blockIdx.x;
+    const double* __restrict__ count, Out o, T* __restrict__ dlogits) {
+  typedef typename Wide<T>::type vec;
+  constexpr int V = Wide<T>::V;
+  __shared__ float red_max[NT / 64];
+  __shared__ double red_sum[NT / 64];
+  __shared__ float given;
+  const int tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
+  // NT = 64: four rows a workgroup, one a wave, no barriers
+  const long row = NT == 64 ? (long)blockIdx.x * 4 +
+                                  __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)
+                            : (long)blockIdx.x;
+  if (row >= r.N) return;
   const float w = weight(r, row);
   if (w == 0.f) {
-    if (threadIdx.x == 0) {
-      if (logp_out) logp_out[row] = 0.f;
-      if (wide_out) wide_out[row] = 0.0;
-      if (stats) stats[row] = make_float2(0.f, 1.f);
+    if (tid == 0) {
+      if (o.logp) o.logp[row] = 0.f;
+      if (o.wide) o.wide[row] = 0.0;
+      if (o.stats) o.stats[row] = make_float2(0.f, 1.f);
       if (POLICY) {
-        row_loss[row] = 0.0;
-        if (dlogits) coef[row] = 0.f, held[row] = 1.f;
+        o.loss[row] = 0.0;
+        if (dlogits) o.coef[row] = 0.f, o.held[row] = 1.f;
       }
     }
     if (POLICY && dlogits)
-      for (int k = threadIdx.x; k < r.K; k += NT)
-        dlogits[row * r.K + k] = (T)0.f;
+      zero_span(dlogits + row * r.K, r.K, 0, r.K, tid, NT);
     return;
   }
   const T* x = logits + row_at(r, row);
-  float m = -INFINITY, s = 0.f;
-  for (int k = threadIdx.x; k < r.K; k += NT) m = fmaxf(m, (float)x[k]);
-  m = group_max<NT>(m, red);
-  for (int k = threadIdx.x; k < r.K; k += NT) s += expf((float)x[k] - m);
-  s = group_sum<NT>(s, red);
   const long y = r.y[row];
   const bool inside = y >= 0 && y < r.K;
-  const double logp = inside ? row_logp((float)x[y], m, s) : (double)NAN;
-  if (threadIdx.x == 0) {
-    if (logp_out) logp_out[row] = (float)logp;
-    if (wide_out) wide_out[row] = logp;
-    if (stats) stats[row] = make_float2(m, s);
+  const float xy = inside ? (float)x[y] : NAN;
+  const int whole = r.K / V, rest = r.K - whole * V;
+  float tail = tid < rest ? (float)x[whole * V + tid] : -INFINITY;
+  constexpr int HELD = E > 0 ? E : 1;
+  vec raw[HELD];
+  float m = tail;
+  Sum sum{0.f, 0.f};
+  if constexpr (E > 0) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (e * NT + tid < whole)
+        raw[e] = *reinterpret_cast<const vec*>(x + (long)(e * NT + tid) * V);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (e * NT + tid < whole) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) m = fmaxf(m, (float)raw[e][i]);
+      }
+    m = group_max<NT>(m, red_max);
+    Sum part[4] = {};  // several chains of additions
+    if (tid < rest) part[0].add(tail, m);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (e * NT + tid < whole) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) part[i & 3].add((float)raw[e][i], m);
+      }
+    part[0].add(part[1]);
+    part[2].add(part[3]);
+    sum = part[0];
+    sum.add(part[2]);
+  } else {
+    // a thread's own maximum and sum; the maximum never holds a NaN, the sum
+    // keeps one
+    m = fmaxf(m, -INFINITY);
+    if (tid < rest) sum.s = tail == tail ? 1.f : NAN;
+    constexpr int U = 4;
+    for (int i0 = tid; i0 < whole; i0 += U * NT) {
+      vec q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * NT < whole)
+          q[u] = *reinterpret_cast<const vec*>(x + (long)(i0 + u * NT) * V);
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * NT < whole) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) top = fmaxf(top, (float)q[u][i]);
+        }
+      // (all minus infinity so far: nothing to move)
+      if (top > m && sum.s != 0.f) sum.move(m, top);
+      m = top;
+      const float at = m == -INFINITY ? 0.f : m;
+      Sum part[4] = {};
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * NT < whole) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) part[i & 3].add((float)q[u][i], at);
+        }
+      part[0].add(part[1]);
+      part[2].add(part[3]);
+      sum.add(part[0]);
+      sum.add(part[2]);
+    }
+    const float all = group_max<NT>(m, red_max);
+    if (m == -INFINITY && all > m) {
+      if (sum.s == sum.s) sum = Sum{0.f, 0.f};
+    } else {
+      sum.move(m, all);
+    }
+    m = all;
+  }
+  const double total_exp = group_sum<NT>(sum.value(), red_sum);
+  const float s = (float)total_exp;
+  float c = 0.f;
+  if (NT == 64 || threadIdx.x < 64) {
+    const double logp = inside ? row_logp(xy, m, total_exp) : (double)NAN;
+    if (tid == 0) {
+      if (o.logp) o.logp[row] = (float)logp;
+      if (o.wide) o.wide[row] = logp;
+      if (o.stats) o.stats[row] = make_float2(m, s);
+    }
+    if constexpr (POLICY) {
+      double loss, slope, total;
+      if (count) {
+        total = *count;
+      } else {
+        // few rows: every row's first wave adds up the weights by itself,
+        // which spares a launch
+        total = 0.0;
+        for (long i = tid; i < r.N; i += 64) total += (double)weight(r, i);
+        total = lanes_sum(total);
+      }
+      policy_row(p, row, r.T, logp, &loss, &slope);
+      const double share = (double)w / fmax(total, 1.0);
+      c = (float)(share * slope);
+      if (tid == 0) {
+        o.loss[row] = share * loss;
+        if (dlogits) o.coef[row] = c, o.held[row] = 1.f;
+      }
+    }
   }
   if constexpr (POLICY) {
-    double loss, slope;
-    policy_row(p, row, r.T, logp, &loss, &slope);
-    const double share = (double)w / fmax(*count, 1.0);
-    if (threadIdx.x == 0) row_loss[row] = share * loss;
-    if (dlogits) {
-      const float c = (float)(share * slope);
-      if (threadIdx.x == 0) coef[row] = c, held[row] = 1.f;
-      const float scale = c / s;
-      for (int k = threadIdx.x; k < r.K; k += NT) {
-        float v = -scale * expf((float)x[k] - m);
-        if (k == y) v += c;
-        dlogits[row * r.K + k] = (T)v;
+    if (!dlogits) return;
+    if constexpr (NT > 64) {
+      if (threadIdx.x == 0) given = c;
+      __syncthreads();
+      c = given;
+    }
+    const float scale = -c / s;
+    T* d = dlogits + row * r.K;
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int i = e * NT + tid;
+        if (i < whole)
+          *reinterpret_cast<vec*>(d + (long)i * V) =
+              grad_of<T>(raw[e], (long)i * V, y, m, scale, c);
       }
+      if (tid < rest) {
+        const int k = whole * V + tid;
+        d[k] = (T)(scale * exp_from(tail, m) + (k == y ? c : 0.f));
+      }
+    } else {
+      grad_span(x, d, r.K, 0, r.K, tid, NT, y, m, scale, c);
     }
   }
 }
 
-// Gradient of rows whose statistics are known.  The row's c is the product of
-// what is given: `coef` a row, `seq` a sequence, its weight (if `weighted`),
-// `up` for all.  held: the factor that the row already holds; such a row is
-// left as it is.
+// c of a row whose statistics are known: the product of what is given, `coef`
+// a row, `seq` a sequence, its weight (if `weighted`), `up` for all.
+struct Factors {
+  const float *coef, *seq, *up;
+  bool weighted;
+};
+
+__device__ __forceinline__ float factor(const Factors& f, const Rows& r,
+                                        uint32_t row, float w) {
+  float c = f.up ? *f.up : 1.f;
+  if (f.coef) c *= f.coef[row];
+  if (f.seq) c *= f.seq[row / (uint32_t)r.T];
+  return f.weighted ? c * w : c;
+}
+
 template <typename T>
-__global__ void rows_grad_kernel(
+__device__ __forceinline__ void grad_row(const T* logits, const Rows& r,
+                                         const float2* stats, const Factors& f,
+                                         long row, int begin, int end,
+                                         int lane, int step, T* dlogits) {
+  const float w = weight(r, row);
+  T* d = dlogits + row * r.K;
+  if (w == 0.f) return zero_span(d, r.K, begin, end, lane, step);
+  const float c = factor(f, r, row, w);
+  const float2 q = stats[row];
+  grad_span(logits + row_at(r, row), d, r.K, begin, end, lane, step, r.y[row],
+            q.x, -c / q.y, c);
+}
+
+// Gradient of rows with known statistics: `lanes` threads and a part of the
+// row each (blockIdx.y), `span` vectors a part.
+template <typename T>
+__global__ __launch_bounds__(256) void rows_grad_kernel(
     const T* __restrict__ logits, Rows r, const float2* __restrict__ stats,
-    const float* __restrict__ coef, const float* __restrict__ seq,
-    bool weighted, const float* __restrict__ up, float* __restrict__ held,
-    T* __restrict__ dlogits) {
-  for (long row = blockIdx.x; row < r.N; row += gridDim.x) {
-    const float w = weight(r, row);
-    const float u = up ? *up : 1.f;
-    if (held && held[row] == u) continue;
-    float c = u;
-    if (coef) c *= coef[row];
-    if (seq) c *= seq[row / r.T];
-    if (weighted) c *= w;
-    T* d = dlogits + row * r.K;
-    if (w == 0.f) {
-      for (int k = threadIdx.x; k < r.K; k += blockDim.x) d[k] = (T)0.f;
-    } else {
-      const T* x = logits + row_at(r, row);
-      const long y = r.y[row];
-      const float2 q = stats[row];
-      const float scale = c / q.y;
-      for (int k = threadIdx.x; k < r.K; k += blockDim.x) {
-        float v = -scale * expf((float)x[k] - q.x);
-        if (k == y) v += c;
-        d[k] = (T)v;
-      }
-    }
-    __syncthreads();
-    if (held && threadIdx.x == 0) held[row] = u;
+    Factors f, int lanes, int span, T* __restrict__ dlogits) {
+  const int sub = threadIdx.x / lanes;
+  const long row = (long)blockIdx.x * (256 / lanes) + sub;
+  if (row >= r.N) return;
+  const int begin = blockIdx.y * span;
+  grad_row(logits, r, stats, f, row, begin, begin + span,
+           (int)threadIdx.x - sub * lanes, lanes, dlogits);
+}
+
+// The same for rows of which some hold this gradient already (`held` is the
+// upstream gradient that a row was made with): those are left as they are.  A
+// workgroup looks at `per` rows at once.
+template <typename T>
+__global__ __launch_bounds__(256) void rows_again_kernel(
+    const T* __restrict__ logits, Rows r, const float2* __restrict__ stats,
+    Factors f, int per, float* __restrict__ held, T* __restrict__ dlogits) {
+  __shared__ int other[64];
+  const long first = (long)blockIdx.x * per;
+  const float up = *f.up;
+  int any = 0;
+  if ((int)threadIdx.x < per) {
+    const long row = first + threadIdx.x;
+    any = row < r.N && !(held[row] == up);
+    other[threadIdx.x] = any;
   }
+  if (!__syncthreads_or(any)) return;
+  for (int i = 0; i < per; ++i)
+    if (other[i])
+      grad_row(logits, r, stats, f, first + i, 0, r.K, (int)threadIdx.x, 256,
+               dlogits);
+  if (any) held[first + threadIdx.x] = up;
 }
 
 // Sum of n values in a fixed order, in 64 bits: one workgroup of 1024.
@@ -273,29 +532,56 @@ Rows rows_of(const torch::Tensor& logits, const torch::Tensor& y,
   return r;
 }
 
+// f(threads a row, vectors a thread) as constants.  A wave for short rows;
+// then as few threads as hold the row in 64 registers each, for more rows at
+// once; 0 vectors: too long to be held.
+template <typename T, bool HOLD, typename F>
+void by_length(int K, F&& f) {
+  constexpr int V = Wide<T>::V;
+  const int v = (K + V - 1) / V;
+  auto at = [&](auto nt, auto e) { f(nt, e); };
+  if (v <= 64) return at(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+  if (v <= 256) return at(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+  if (v <= 1024) return at(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
+  if constexpr (HOLD) {
+    if (v <= 2048) return at(std::integral_constant<int, 256>(), std::integral_constant<int, 8>());
+    if (v <= 4096) return at(std::integral_constant<int, 256>(), std::integral_constant<int, 16>());
+    if (v <= 8192) return at(std::integral_constant<int, 512>(), std::integral_constant<int, 16>());
+    if (v <= 16384) return at(std::integral_constant<int, 1024>(), std::integral_constant<int, 16>());
+  }
+  at(std::integral_constant<int, 256>(), std::integral_constant<int, 0>());
+}
+
 template <bool POLICY>
 void launch_rows(const torch::Tensor& logits, const Rows& r, const Policy& p,
-                 const double* count, float* logp, double* wide,
-                 float2* stats, double* row_loss, float* coef, float* held, void* dlogits) {
+                 const double* count, const Out& o, void* dlogits) {
   by_type(logits, "seqloss", [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    hipLaunchKernelGGL((rows_kernel<T, 256, POLICY>), dim3(r.N), dim3(256), 0,
-                       stream_of(logits), data<T>(logits), r, p, count, logp,
-                       wide, stats, row_loss, coef, held, (T*)dlogits);
+    by_length<T, POLICY>(r.K, [&](auto nt, auto e) {
+      constexpr int NT = decltype(nt)::value, E = decltype(e)::value;
+      const long groups = NT == 64 ? (r.N + 3) / 4 : r.N;
+      hipLaunchKernelGGL((rows_kernel<T, NT, E, POLICY>), dim3(groups),
+                         dim3(NT < 256 ? 256 : NT), 0, stream_of(logits),
+                         data<T>(logits), r, p, count, o, (T*)dlogits);
+    });
   });
   launched("seqloss");
 }
 
 void launch_grad(const torch::Tensor& logits, const Rows& r,
-                 const torch::Tensor& stats, const float* coef,
-                 const float* seq, bool weighted, const float* up, float* held,
+                 const torch::Tensor& stats, const Factors& f,
                  torch::Tensor& dlogits) {
   by_type(logits, "seqloss", [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    hipLaunchKernelGGL(rows_grad_kernel<T>, dim3(std::min(r.N, 4096L)),
-                       dim3(256), 0, stream_of(logits), data<T>(logits), r,
-                       data<float2>(stats), coef, seq, weighted, up, held,
-                       data<T>(dlogits));
+    const int v = r.K / Wide<T>::V + 1;  // with the rest of the row
+    int lanes = 16;
+    while (lanes < 256 && lanes < v) lanes *= 2;
+    const int span = 256 * 8;
+    const long groups = (r.N * lanes + 255) / 256;
+    hipLaunchKernelGGL(rows_grad_kernel<T>,
+                       dim3(groups, (v + span - 1) / span), dim3(256), 0,
+                       stream_of(logits), data<T>(logits), r,
+                       data<float2>(stats), f, lanes, span, data<T>(dlogits));
   });
   launched("seqloss gradient");
 }
@@ -310,8 +596,9 @@ std::vector<torch::Tensor> token_logprob_fwd(
   const auto f32 = logits.options().dtype(at::kFloat);
   auto logp = torch::empty({logits.size(0), logits.size(1)}, f32);
   auto stats = torch::empty({r.N, 2}, f32);
-  launch_rows<false>(logits, r, Policy{}, nullptr, data<float>(logp), nullptr,
-                     data<float2>(stats), nullptr, nullptr, nullptr, nullptr);
+  launch_rows<false>(logits, r, Policy{}, nullptr,
+                     Out{data<float>(logp), nullptr, data<float2>(stats)},
+                     nullptr);
   return {logp, stats};
 }
 
@@ -326,8 +613,7 @@ torch::Tensor token_logprob_bwd(
   TORCH_CHECK(dlogp.numel() == r.N && stats.numel() == 2 * r.N);
   c10::DeviceGuard guard(logits.device());
   auto d = torch::empty(logits.sizes(), logits.options());
-  launch_grad(logits, r, stats, data<float>(dlogp), nullptr, false, nullptr,
-              nullptr, d);
+  launch_grad(logits, r, stats, Factors{data<float>(dlogp)}, d);
   return d;
 }
 
@@ -367,12 +653,15 @@ std::vector<torch::Tensor> policy_loss_fwd(
     coef = torch::empty({r.N}, f32);
     held = torch::empty({r.N}, f32);
   }
-  hipLaunchKernelGGL((sum_kernel<float, double>), dim3(1), dim3(1024), 0,
-                     stream_of(logits), r.w, r.N, count);
-  launch_rows<true>(logits, r, p, count, data<float>(logp), nullptr,
-                    grad ? data<float2>(stats) : nullptr, row_loss,
-                    grad ? data<float>(coef) : nullptr,
-                    grad ? data<float>(held) : nullptr,
+  const bool few = r.N <= 1024;
+  if (!few)
+    hipLaunchKernelGGL((sum_kernel<float, double>), dim3(1), dim3(1024), 0,
+                       stream_of(logits), r.w, r.N, count);
+  launch_rows<true>(logits, r, p, few ? nullptr : count,
+                    Out{data<float>(logp), nullptr,
+                        grad ? data<float2>(stats) : nullptr, row_loss,
+                        grad ? data<float>(coef) : nullptr,
+                        grad ? data<float>(held) : nullptr},
                     grad ? dlogits.data_ptr() : nullptr);
   hipLaunchKernelGGL((sum_kernel<double, float>), dim3(1), dim3(1024), 0,
                      stream_of(logits), row_loss, r.N, data<float>(loss));
@@ -401,8 +690,17 @@ void policy_loss_bwd(
     TORCH_CHECK(held->numel() == r.N);
   }
   c10::DeviceGuard guard(logits.device());
-  launch_grad(logits, r, stats, data<float>(coef), nullptr, false,
-              data<float>(up), data_or_null<float>(held), dlogits);
+  const Factors f{data<float>(coef), nullptr, data<float>(up), false};
+  if (!held.has_value()) return launch_grad(logits, r, stats, f, dlogits);
+  const int per = std::min((r.N + 2047) / 2048, 64L);
+  by_type(logits, "policy_loss", [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    hipLaunchKernelGGL(rows_again_kernel<T>, dim3((r.N + per - 1) / per),
+                       dim3(256), 0, stream_of(logits), data<T>(logits), r,
+                       data<float2>(stats), f, per, data<float>(*held),
+                       data<T>(dlogits));
+  });
+  launched("policy_loss gradient");
 }
 
 // -> loss, margins [P], and for the backward pass: stats, d loss / d gain [2P].
@@ -423,8 +721,9 @@ std::vector<torch::Tensor> preference_loss_fwd(
   auto stats = torch::empty({r.N, 2}, f32);
   auto gain = torch::empty({B}, f32.dtype(at::kDouble));
   auto seq = torch::empty({B}, f32);
-  launch_rows<false>(logits, r, Policy{}, nullptr, nullptr, data<double>(logp),
-                     data<float2>(stats), nullptr, nullptr, nullptr, nullptr);
+  launch_rows<false>(logits, r, Policy{}, nullptr,
+                     Out{nullptr, data<double>(logp), data<float2>(stats)},
+                     nullptr);
   hipLaunchKernelGGL(gain_kernel, dim3(B), dim3(256), 0, stream_of(logits),
                      data<double>(logp), data<float>(ref), r,
                      data<double>(gain));
@@ -446,7 +745,7 @@ torch::Tensor preference_loss_bwd(
               seq.numel() == logits.size(0));
   c10::DeviceGuard guard(logits.device());
   auto d = torch::empty(logits.sizes(), logits.options());
-  launch_grad(logits, r, stats, nullptr, data<float>(seq), true,
-              data<float>(up), nullptr, d);
+  launch_grad(logits, r, stats,
+              Factors{nullptr, data<float>(seq), data<float>(up), true}, d);
   return d;
 }
