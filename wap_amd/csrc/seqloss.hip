@@ -48,6 +48,26 @@ struct Wide {
   typedef typename VecOf<T, V, sizeof(T)>::type type;
 };
 
+// A row as `whole` vectors of 16 bytes from its first element on, wherever that
+// lies (rows of 50001 f32 tokens read at 5.6 TB/s, rows of 50000 at 5.7; and a
+// sum does not depend on the place), and the `rest` behind them, one a lane.
+template <typename T>
+struct Cut {
+  int whole, rest;
+
+  __device__ __forceinline__ explicit Cut(int K) {
+    whole = K / Wide<T>::V;
+    rest = K - whole * Wide<T>::V;
+  }
+  // token of vector i, and of a lane of the rest
+  __device__ __forceinline__ long vec_at(int i) const {
+    return (long)i * Wide<T>::V;
+  }
+  __device__ __forceinline__ int rest_at(int lane) const {
+    return whole * Wide<T>::V + lane;
+  }
+};
+
 constexpr float LOG2E = 1.44269502162933349609f;
 // log2 e = LOG2E (1 + LOST)
 constexpr double LOST = 1.92596299112661746887e-8 / 1.44269502162933349609;
@@ -141,6 +161,17 @@ __device__ __forceinline__ void policy_row(
   }
 }
 
+// Stores past the caches where `cold`: a gradient larger than the 256 MB of
+// the last cache would only push out what is still to be read (8192 x 32768
+// bf16 policy: 191 us, 205 with plain stores); a smaller one is read from there next.
+template <bool COLD, typename V>
+__device__ __forceinline__ void put(V* p, const V& v) {
+  if constexpr (COLD)
+    __builtin_nontemporal_store(v, p);
+  else
+    *p = v;
+}
+
 // Where a row's results go.
 struct Out {
   float* logp;       // or null
@@ -170,39 +201,39 @@ __device__ __forceinline__ typename Wide<T>::type grad_of(
   return d;
 }
 
-// The gradient of a row's vectors begin + lane, + step, .. below end.  What is
-// left of a row that is no multiple of V goes with the part that the next
-// vector would be in.
-template <typename T>
+// The gradient of a row's vectors begin + lane, + step, .. below end; the
+// part that begins at 0 has the rest of the row.
+template <bool COLD, typename T>
 __device__ __forceinline__ void grad_span(const T* x, T* d, int K, int begin,
                                           int end, int lane, int step, long y,
                                           float m, float scale, float c) {
   typedef typename Wide<T>::type vec;
-  constexpr int V = Wide<T>::V;
-  const int whole = K / V;
-  for (int i = begin + lane; i < end && i < whole; i += step)
-    *reinterpret_cast<vec*>(d + (long)i * V) = grad_of<T>(
-        *reinterpret_cast<const vec*>(x + (long)i * V), (long)i * V, y, m,
-        scale, c);
-  const int k = whole * V + lane;
-  if (k < K && begin <= whole && whole < end)
+  const Cut<T> cut(K);
+  for (int i = begin + lane; i < end && i < cut.whole; i += step) {
+    const long k = cut.vec_at(i);
+    put<COLD>(
+        reinterpret_cast<vec*>(d + k),
+        grad_of<T>(*reinterpret_cast<const vec*>(x + k), k, y, m, scale, c));
+  }
+  if (begin == 0 && lane < cut.rest) {
+    const int k = cut.rest_at(lane);
     d[k] = (T)(scale * exp_from((float)x[k], m) + (k == y ? c : 0.f));
+  }
 }
 
-template <typename T>
+template <bool COLD, typename T>
 __device__ __forceinline__ void zero_span(T* d, int K, int begin, int end,
                                           int lane, int step) {
   typedef typename Wide<T>::type vec;
   constexpr int V = Wide<T>::V;
-  const int whole = K / V;
-  for (int i = begin + lane; i < end && i < whole; i += step) {
+  const Cut<T> cut(K);
+  for (int i = begin + lane; i < end && i < cut.whole; i += step) {
     vec z;
 #pragma unroll
     for (int j = 0; j < V; ++j) z[j] = (T)0.f;
-    *reinterpret_cast<vec*>(d + (long)i * V) = z;
+    put<COLD>(reinterpret_cast<vec*>(d + cut.vec_at(i)), z);
   }
-  if (whole * V + lane < K && begin <= whole && whole < end)
-    d[whole * V + lane] = (T)0.f;
+  if (begin == 0 && lane < cut.rest) d[cut.rest_at(lane)] = (T)0.f;
 }
 
 // Rows of logits to logp, and with POLICY to the loss and, if `dlogits`, its
@@ -215,7 +246,7 @@ __device__ __forceinline__ void zero_span(T* d, int K, int begin, int end,
 // for the sums (a running maximum and sum a thread) and again for the
 // gradient.  Bound by memory: 18 instruction slots an element of bf16 are 0.4
 // of what reading and writing it takes.
-template <typename T, int NT, int E, bool POLICY>
+template <typename T, int NT, int E, bool POLICY, bool COLD>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
     const T* __restrict__ logits, Rows r, Policy p,
     const double* __restrict__ count, Out o, T* __restrict__ dlogits) {
@@ -242,15 +273,16 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
       }
     }
     if (POLICY && dlogits)
-      zero_span(dlogits + row * r.K, r.K, 0, r.K, tid, NT);
+      zero_span<COLD>(dlogits + row * r.K, r.K, 0, r.K, tid, NT);
     return;
   }
   const T* x = logits + row_at(r, row);
   const long y = r.y[row];
   const bool inside = y >= 0 && y < r.K;
   const float xy = inside ? (float)x[y] : NAN;
-  const int whole = r.K / V, rest = r.K - whole * V;
-  float tail = tid < rest ? (float)x[whole * V + tid] : -INFINITY;
+  const Cut<T> cut(r.K);
+  const int whole = cut.whole, rest = cut.rest;
+  float tail = tid < rest ? (float)x[cut.rest_at(tid)] : -INFINITY;
   constexpr int HELD = E > 0 ? E : 1;
   vec raw[HELD];
   float m = tail;
@@ -259,7 +291,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (e * NT + tid < whole)
-        raw[e] = *reinterpret_cast<const vec*>(x + (long)(e * NT + tid) * V);
+        raw[e] = *reinterpret_cast<const vec*>(x + cut.vec_at(e * NT + tid));
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (e * NT + tid < whole) {
@@ -290,7 +322,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (i0 + u * NT < whole)
-          q[u] = *reinterpret_cast<const vec*>(x + (long)(i0 + u * NT) * V);
+          q[u] = *reinterpret_cast<const vec*>(x + cut.vec_at(i0 + u * NT));
       float top = m;
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -366,15 +398,15 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
       for (int e = 0; e < E; ++e) {
         const int i = e * NT + tid;
         if (i < whole)
-          *reinterpret_cast<vec*>(d + (long)i * V) =
-              grad_of<T>(raw[e], (long)i * V, y, m, scale, c);
+          put<COLD>(reinterpret_cast<vec*>(d + cut.vec_at(i)),
+                    grad_of<T>(raw[e], cut.vec_at(i), y, m, scale, c));
       }
       if (tid < rest) {
-        const int k = whole * V + tid;
+        const int k = cut.rest_at(tid);
         d[k] = (T)(scale * exp_from(tail, m) + (k == y ? c : 0.f));
       }
     } else {
-      grad_span(x, d, r.K, 0, r.K, tid, NT, y, m, scale, c);
+      grad_span<COLD>(x, d, r.K, 0, r.K, tid, NT, y, m, scale, c);
     }
   }
 }
@@ -394,23 +426,23 @@ __device__ __forceinline__ float factor(const Factors& f, const Rows& r,
   return f.weighted ? c * w : c;
 }
 
-template <typename T>
+template <bool COLD, typename T>
 __device__ __forceinline__ void grad_row(const T* logits, const Rows& r,
                                          const float2* stats, const Factors& f,
                                          long row, int begin, int end,
                                          int lane, int step, T* dlogits) {
   const float w = weight(r, row);
   T* d = dlogits + row * r.K;
-  if (w == 0.f) return zero_span(d, r.K, begin, end, lane, step);
+  if (w == 0.f) return zero_span<COLD>(d, r.K, begin, end, lane, step);
   const float c = factor(f, r, row, w);
   const float2 q = stats[row];
-  grad_span(logits + row_at(r, row), d, r.K, begin, end, lane, step, r.y[row],
-            q.x, -c / q.y, c);
+  grad_span<COLD>(logits + row_at(r, row), d, r.K, begin, end, lane, step,
+                  r.y[row], q.x, -c / q.y, c);
 }
 
 // Gradient of rows with known statistics: `lanes` threads and a part of the
 // row each (blockIdx.y), `span` vectors a part.
-template <typename T>
+template <typename T, bool COLD>
 __global__ __launch_bounds__(256) void rows_grad_kernel(
     const T* __restrict__ logits, Rows r, const float2* __restrict__ stats,
     Factors f, int lanes, int span, T* __restrict__ dlogits) {
@@ -418,7 +450,7 @@ __global__ __launch_bounds__(256) void rows_grad_kernel(
   const long row = (long)blockIdx.x * (256 / lanes) + sub;
   if (row >= r.N) return;
   const int begin = blockIdx.y * span;
-  grad_row(logits, r, stats, f, row, begin, begin + span,
+  grad_row<COLD>(logits, r, stats, f, row, begin, begin + span,
            (int)threadIdx.x - sub * lanes, lanes, dlogits);
 }
 
@@ -441,7 +473,7 @@ __global__ __launch_bounds__(256) void rows_again_kernel(
   if (!__syncthreads_or(any)) return;
   for (int i = 0; i < per; ++i)
     if (other[i])
-      grad_row(logits, r, stats, f, first + i, 0, r.K, (int)threadIdx.x, 256,
+      grad_row<false>(logits, r, stats, f, first + i, 0, r.K, (int)threadIdx.x, 256,
                dlogits);
   if (any) held[first + threadIdx.x] = up;
 }
@@ -458,12 +490,16 @@ __device__ __forceinline__ double wide_sum(double v, double* red) {
 }
 
 template <typename V, typename O>
-__global__ void sum_kernel(const V* __restrict__ v, long n,
+__global__ __launch_bounds__(1024) void sum_kernel(const V* __restrict__ v, long n,
                            O* __restrict__ out) {
   __shared__ double red[16];
-  double s = 0.0;
-  for (long i = threadIdx.x; i < n; i += blockDim.x) s += (double)v[i];
-  s = wide_sum(s, red);
+  // four loads on their way at once: the time is all latency
+  double part[4] = {0.0, 0.0, 0.0, 0.0};
+  for (long i = threadIdx.x; i < n; i += 4 * 1024)
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u * 1024 < n) part[u] += (double)v[i + u * 1024];
+  const double s = wide_sum((part[0] + part[1]) + (part[2] + part[3]), red);
   if (threadIdx.x == 0) *out = (O)s;
 }
 
@@ -483,18 +519,18 @@ __global__ void gain_kernel(const double* __restrict__ logp,
 }
 
 // loss = mean_i (1 - eps) softplus(-margin_i) + eps softplus(margin_i), and
-// every sequence's d loss / d gain.
-__global__ void pairs_kernel(const double* __restrict__ gain, long P,
-                             double beta, double eps, float* __restrict__ loss,
-                             float* __restrict__ margin,
-                             float* __restrict__ seq) {
-  __shared__ double red[16];
+// every sequence's d loss / d gain, by one workgroup.
+__device__ __forceinline__ void pairs_loss(const double* gain, long P,
+                                           double beta, double eps,
+                                           float* loss, float* margin,
+                                           float* seq, double* red) {
   double s = 0.0;
   for (long i = threadIdx.x; i < P; i += blockDim.x) {
     const double m = beta * (gain[i] - gain[P + i]);
-    const double soft = log1p(exp(-fabs(m)));
+    const double e = exp(-fabs(m)), soft = log1p(e), big = 1.0 / (1.0 + e);
     s += (1.0 - eps) * (soft + fmax(-m, 0.0)) + eps * (soft + fmax(m, 0.0));
-    const double up = 1.0 / (1.0 + exp(-m)), down = 1.0 / (1.0 + exp(m));
+    // sigmoid(m), sigmoid(-m) from the one exponential
+    const double up = m >= 0.0 ? big : e * big, down = m >= 0.0 ? e * big : big;
     const double d = beta * (eps * up - (1.0 - eps) * down) / (double)P;
     margin[i] = (float)m;
     seq[i] = (float)d;
@@ -502,6 +538,39 @@ __global__ void pairs_kernel(const double* __restrict__ gain, long P,
   }
   s = wide_sum(s, red);
   if (threadIdx.x == 0) *loss = (float)(s / (double)P);
+}
+
+__global__ void pairs_kernel(const double* __restrict__ gain, long P,
+                             double beta, double eps, float* __restrict__ loss,
+                             float* __restrict__ margin,
+                             float* __restrict__ seq) {
+  __shared__ double red[16];
+  pairs_loss(gain, P, beta, eps, loss, margin, seq, red);
+}
+
+// Both at once for few tokens: a wave a sequence, up to FEW_SEQS of them.
+constexpr int FEW_SEQS = 256;
+
+__global__ __launch_bounds__(1024) void gain_pairs_kernel(
+    const double* __restrict__ logp, const float* __restrict__ ref, Rows r,
+    long P, double beta, double eps, float* __restrict__ loss,
+    float* __restrict__ margin, float* __restrict__ seq) {
+  __shared__ double red[16];
+  __shared__ double gain[FEW_SEQS];
+  const int lane = threadIdx.x & 63;
+  for (long b = threadIdx.x >> 6; b < 2 * P; b += 16) {
+    double s = 0.0;
+    for (long t = lane; t < r.T; t += 64) {
+      const long i = b * r.T + t;
+      const float w = weight(r, i);
+      const double got = logp[i], was = (double)ref[i];
+      if (w != 0.f) s += (double)w * (got - was);
+    }
+    s = lanes_sum(s);
+    if (lane == 0) gain[b] = s;
+  }
+  __syncthreads();
+  pairs_loss(gain, P, beta, eps, loss, margin, seq, red);
 }
 
 Rows rows_of(const torch::Tensor& logits, const torch::Tensor& y,
@@ -532,9 +601,20 @@ Rows rows_of(const torch::Tensor& logits, const torch::Tensor& y,
   return r;
 }
 
+// f(true) for gradients that are stored past the caches.
+template <typename F>
+void by_size(const torch::Tensor& logits, F&& f) {
+  if (logits.numel() * logits.element_size() > (256L << 20))
+    f(std::true_type());
+  else
+    f(std::false_type());
+}
+
 // f(threads a row, vectors a thread) as constants.  A wave for short rows;
 // then as few threads as hold the row in 64 registers each, for more rows at
-// once; 0 vectors: too long to be held.
+// once (8192 x 32768 bf16 policy: 191 us with 256 or 512 threads a row, 193
+// with 1024); 0 vectors: too long to be held, or nothing to hold it for (4096 x
+// 131072 bf16 logprob, 2616 rows that count: 134 us with 512, 139 with 256).
 template <typename T, bool HOLD, typename F>
 void by_length(int K, F&& f) {
   constexpr int V = Wide<T>::V;
@@ -549,7 +629,7 @@ void by_length(int K, F&& f) {
     if (v <= 8192) return at(std::integral_constant<int, 512>(), std::integral_constant<int, 16>());
     if (v <= 16384) return at(std::integral_constant<int, 1024>(), std::integral_constant<int, 16>());
   }
-  at(std::integral_constant<int, 256>(), std::integral_constant<int, 0>());
+  at(std::integral_constant<int, 512>(), std::integral_constant<int, 0>());
 }
 
 template <bool POLICY>
@@ -560,9 +640,16 @@ void launch_rows(const torch::Tensor& logits, const Rows& r, const Policy& p,
     by_length<T, POLICY>(r.K, [&](auto nt, auto e) {
       constexpr int NT = decltype(nt)::value, E = decltype(e)::value;
       const long groups = NT == 64 ? (r.N + 3) / 4 : r.N;
-      hipLaunchKernelGGL((rows_kernel<T, NT, E, POLICY>), dim3(groups),
-                         dim3(NT < 256 ? 256 : NT), 0, stream_of(logits),
-                         data<T>(logits), r, p, count, o, (T*)dlogits);
+      auto go = [&](auto cold) {
+        hipLaunchKernelGGL(
+            (rows_kernel<T, NT, E, POLICY, decltype(cold)::value>),
+            dim3(groups), dim3(NT < 256 ? 256 : NT), 0, stream_of(logits),
+            data<T>(logits), r, p, count, o, (T*)dlogits);
+      };
+      if constexpr (POLICY)
+        by_size(logits, go);
+      else
+        go(std::false_type());
     });
   });
   launched("seqloss");
@@ -578,10 +665,13 @@ void launch_grad(const torch::Tensor& logits, const Rows& r,
     while (lanes < 256 && lanes < v) lanes *= 2;
     const int span = 256 * 8;
     const long groups = (r.N * lanes + 255) / 256;
-    hipLaunchKernelGGL(rows_grad_kernel<T>,
-                       dim3(groups, (v + span - 1) / span), dim3(256), 0,
-                       stream_of(logits), data<T>(logits), r,
-                       data<float2>(stats), f, lanes, span, data<T>(dlogits));
+    by_size(logits, [&](auto cold) {
+      hipLaunchKernelGGL((rows_grad_kernel<T, decltype(cold)::value>),
+                         dim3(groups, (v + span - 1) / span), dim3(256), 0,
+                         stream_of(logits), data<T>(logits), r,
+                         data<float2>(stats), f, lanes, span,
+                         data<T>(dlogits));
+    });
   });
   launched("seqloss gradient");
 }
@@ -719,17 +809,25 @@ std::vector<torch::Tensor> preference_loss_fwd(
   // 64-bit: a gain is a small difference of long sums
   auto logp = torch::empty({r.N}, f32.dtype(at::kDouble));
   auto stats = torch::empty({r.N, 2}, f32);
-  auto gain = torch::empty({B}, f32.dtype(at::kDouble));
   auto seq = torch::empty({B}, f32);
   launch_rows<false>(logits, r, Policy{}, nullptr,
                      Out{nullptr, data<double>(logp), data<float2>(stats)},
                      nullptr);
-  hipLaunchKernelGGL(gain_kernel, dim3(B), dim3(256), 0, stream_of(logits),
-                     data<double>(logp), data<float>(ref), r,
-                     data<double>(gain));
-  hipLaunchKernelGGL(pairs_kernel, dim3(1), dim3(256), 0, stream_of(logits),
-                     data<double>(gain), B / 2, beta, eps, data<float>(loss),
-                     data<float>(margin), data<float>(seq));
+  // a second launch takes about 5 us; one workgroup reads 16384 tokens in that
+  if (r.N <= 16384 && B <= FEW_SEQS) {
+    hipLaunchKernelGGL(gain_pairs_kernel, dim3(1), dim3(1024), 0,
+                       stream_of(logits), data<double>(logp), data<float>(ref),
+                       r, B / 2, beta, eps, data<float>(loss),
+                       data<float>(margin), data<float>(seq));
+  } else {
+    auto gain = torch::empty({B}, logp.options());
+    hipLaunchKernelGGL(gain_kernel, dim3(B), dim3(256), 0, stream_of(logits),
+                       data<double>(logp), data<float>(ref), r,
+                       data<double>(gain));
+    hipLaunchKernelGGL(pairs_kernel, dim3(1), dim3(256), 0, stream_of(logits),
+                       data<double>(gain), B / 2, beta, eps, data<float>(loss),
+                       data<float>(margin), data<float>(seq));
+  }
   launched("preference_loss");
   return {loss, margin, stats, seq};
 }
