@@ -103,7 +103,7 @@ __global__ __launch_bounds__(THREADS) void ctr_dropout_kernel(
 // device, or the two numbers.  Returns y and, where rng is a tensor, the seed
 // and step that were used: the backward pass draws from that copy, whatever
 // the caller has done to rng since.
-std::vector<torch::Tensor> counter_dropout(
+std::vector<torch::Tensor> counter_dropout_run(
     torch::Tensor x, c10::optional<torch::Tensor> residual, double p,
     c10::optional<torch::Tensor> rng, int64_t seed, int64_t step,
     int64_t stream, bool keep_used) {

@@ -849,7 +849,8 @@ std::vector<torch::Tensor> gated_scan_bwd(
   return {dg};
 }
 
-std::vector<torch::Tensor> gated_step(torch::Tensor g, torch::Tensor h) {
+std::tuple<torch::Tensor, torch::Tensor> gated_step_run(torch::Tensor g,
+                                                        torch::Tensor h) {
   check_gates(g, 2);
   check_state(h, g);
   c10::DeviceGuard guard(g.device());

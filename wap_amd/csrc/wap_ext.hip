@@ -923,43 +923,25 @@ torch::Tensor bnrelu_conv_fwd_mxfp8(
   return out;
 }
 
-// gated linear recurrence (gscan.hip)
-std::vector<torch::Tensor> gated_scan_fwd(
+// sequence operators (seqops.cpp over gscan.hip, seqloss.hip, ctrdrop.hip)
+std::tuple<torch::Tensor, torch::Tensor> gated_scan(
     torch::Tensor g, c10::optional<torch::Tensor> h0,
-    c10::optional<torch::Tensor> mask, bool keep);
-std::vector<torch::Tensor> gated_scan_bwd(
-    torch::Tensor g, c10::optional<torch::Tensor> h0,
-    c10::optional<torch::Tensor> mask, c10::optional<torch::Tensor> marks,
-    c10::optional<torch::Tensor> dh, c10::optional<torch::Tensor> dlast);
-std::vector<torch::Tensor> gated_step(torch::Tensor g, torch::Tensor h);
-
-// token probabilities and sequence losses (seqloss.hip)
-std::vector<torch::Tensor> token_logprob_fwd(
-    torch::Tensor logits, torch::Tensor y, c10::optional<torch::Tensor> w);
-torch::Tensor token_logprob_bwd(
-    torch::Tensor logits, torch::Tensor y, c10::optional<torch::Tensor> w,
-    torch::Tensor stats, torch::Tensor dlogp);
-std::vector<torch::Tensor> policy_loss_fwd(
-    torch::Tensor logits, torch::Tensor y, torch::Tensor w,
-    torch::Tensor old_logp, torch::Tensor adv,
-    c10::optional<torch::Tensor> ref, double lo, double hi, double beta,
-    bool grad);
-void policy_loss_bwd(
-    torch::Tensor logits, torch::Tensor y, torch::Tensor w,
-    torch::Tensor stats, torch::Tensor coef, c10::optional<torch::Tensor> held,
-    torch::Tensor up, torch::Tensor dlogits);
-std::vector<torch::Tensor> preference_loss_fwd(
-    torch::Tensor logits, torch::Tensor y, torch::Tensor w, torch::Tensor ref,
-    double beta, double eps);
-torch::Tensor preference_loss_bwd(
-    torch::Tensor logits, torch::Tensor y, torch::Tensor w,
-    torch::Tensor stats, torch::Tensor seq, torch::Tensor up);
-
-// counter-based dropout (ctrdrop.hip)
-std::vector<torch::Tensor> counter_dropout(
+    c10::optional<torch::Tensor> mask);
+std::tuple<torch::Tensor, torch::Tensor> gated_step(
+    torch::Tensor g, torch::Tensor h);
+torch::Tensor token_logprob(
+    torch::Tensor logits, torch::Tensor y, c10::optional<torch::Tensor> mask);
+std::tuple<torch::Tensor, torch::Tensor> policy_loss(
+    torch::Tensor logits, torch::Tensor y, torch::Tensor mask,
+    torch::Tensor old_logp, torch::Tensor advantage,
+    c10::optional<torch::Tensor> ref_logp, double lo, double hi, double beta);
+std::tuple<torch::Tensor, torch::Tensor> preference_loss(
+    torch::Tensor logits, torch::Tensor y, torch::Tensor mask,
+    torch::Tensor ref_logp, double beta, double eps);
+torch::Tensor counter_dropout(
     torch::Tensor x, c10::optional<torch::Tensor> residual, double p,
     c10::optional<torch::Tensor> rng, int64_t seed, int64_t step,
-    int64_t stream, bool keep_used);
+    int64_t stream);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bnrelu_conv_fwd_mxfp8", &bnrelu_conv_fwd_mxfp8);
@@ -986,15 +968,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gru_gates_fwd", &gru_gates_fwd);
   m.def("gru_gates_bwd", &gru_gates_bwd);
   m.def("fused_gru_cell", &fused_gru_cell);
-  m.def("gated_scan_fwd", &gated_scan_fwd);
-  m.def("gated_scan_bwd", &gated_scan_bwd);
+  m.def("gated_scan", &gated_scan);
   m.def("gated_step", &gated_step);
-  m.def("token_logprob_fwd", &token_logprob_fwd);
-  m.def("token_logprob_bwd", &token_logprob_bwd);
-  m.def("policy_loss_fwd", &policy_loss_fwd);
-  m.def("policy_loss_bwd", &policy_loss_bwd);
-  m.def("preference_loss_fwd", &preference_loss_fwd);
-  m.def("preference_loss_bwd", &preference_loss_bwd);
+  m.def("token_logprob", &token_logprob);
+  m.def("policy_loss", &policy_loss);
+  m.def("preference_loss", &preference_loss);
   m.def("counter_dropout", &counter_dropout);
   m.attr("arch") = "gfx950";
 }

@@ -15,7 +15,7 @@ replay.
 from __future__ import annotations
 
 import math
-from typing import Optional, Sequence, Tuple, Union
+from typing import Optional, Sequence, Union
 
 import torch
 from torch import Tensor
@@ -51,27 +51,16 @@ def _draws(n: int, rng: Tensor, stream: int) -> Tensor:
     return torch.stack([words & 0xFFFF, words >> 16], dim=-1).view(-1)[:n]
 
 
-def _apply(x: Tensor, residual: Optional[Tensor], p: float,
-           rng: Union[Tensor, Tuple[int, int]], stream: int, keep: bool):
-    """(y, the seed and step that were used) of a contiguous x."""
-    if _hip(x):
-        from . import ext
-        if isinstance(rng, Tensor):
-            out = ext.require().counter_dropout(x, residual, p, rng, 0, 0,
-                                                stream, keep)
-            return out[0], (out[1] if keep else None)
-        y, = ext.require().counter_dropout(x, residual, p, None, rng[0],
-                                           rng[1], stream, False)
-        return y, rng
-    at = (rng.clone() if isinstance(rng, Tensor)
-          else torch.tensor(rng, dtype=torch.int64, device=x.device))
+def _apply(x: Tensor, residual: Optional[Tensor], p: float, rng: Tensor,
+           stream: int) -> Tensor:
+    """Of a contiguous x (eager; the HIP path has its own node)."""
     limit = _limit(p)
-    on = (_draws(x.numel(), at, stream) >= limit).view(x.shape)
+    on = (_draws(x.numel(), rng, stream) >= limit).view(x.shape)
     scale = 65536 / (65536 - limit) if limit < 65536 else 0.0
     y = torch.where(on, _up(x) * scale, 0.0)
     if residual is not None:
         y = y + _up(residual)
-    return y.to(x.dtype), (at if isinstance(rng, Tensor) else rng)
+    return y.to(x.dtype)
 
 
 def _in_order(t: Tensor, fmt: Optional[torch.memory_format]) -> Tensor:
@@ -97,17 +86,13 @@ class _CounterDropout(torch.autograd.Function):
             last = {4: torch.channels_last, 5: torch.channels_last_3d}.get(x.dim())
             if last is not None and x.is_contiguous(memory_format=last):
                 fmt = last
-        keep = ctx.needs_input_grad[0]
-        y, used = _apply(_in_order(x.detach(), fmt),
-                         None if residual is None
-                         else _in_order(residual.detach(), fmt),
-                         p, rng, stream, keep)
+        rng = (rng.clone() if isinstance(rng, Tensor)
+               else torch.tensor(rng, dtype=torch.int64, device=x.device))
+        y = _apply(_in_order(x, fmt),
+                   None if residual is None else _in_order(residual, fmt),
+                   p, rng, stream)
         ctx.meta = (p, stream, fmt, residual is not None)
-        ctx.used = None
-        if isinstance(used, Tensor):
-            ctx.save_for_backward(used)
-        else:
-            ctx.used = used
+        ctx.save_for_backward(rng)
         return _back(y, fmt)
 
     @staticmethod
@@ -116,9 +101,8 @@ class _CounterDropout(torch.autograd.Function):
         p, stream, fmt, has_res = ctx.meta
         dx = None
         if ctx.needs_input_grad[0]:
-            used = ctx.used if ctx.used is not None else ctx.saved_tensors[0]
-            dx, _ = _apply(_in_order(dy, fmt), None, p, used, stream, False)
-            dx = _back(dx, fmt)
+            rng, = ctx.saved_tensors
+            dx = _back(_apply(_in_order(dy, fmt), None, p, rng, stream), fmt)
         dres = dy if has_res and ctx.needs_input_grad[1] else None
         return dx, dres, None, None, None
 
@@ -149,15 +133,21 @@ def counter_dropout(x: Tensor, p: float, rng: Union[Tensor, Sequence[int]],
         raise ValueError(f"counter_dropout: p must be in [0, 1], got {p}")
     if not 0 <= stream < 1 << 24:
         raise ValueError(f"counter_dropout: stream must be in [0, 2**24), got {stream}")
+    at = None
     if isinstance(rng, Tensor):
-        if rng.dtype != torch.int64 or tuple(rng.shape) != (2,) or rng.device != x.device:
-            raise ValueError("counter_dropout: rng must be int64 [2] on "
-                             f"{x.device}, got {rng.dtype} {tuple(rng.shape)} on {rng.device}")
-        rng = rng.detach().contiguous()
-    else:
-        if len(rng) != 2:
-            raise ValueError("counter_dropout: rng must be (seed, step)")
+        at = rng
+    elif len(rng) == 2:
         rng = (_signed(int(rng[0])), _signed(int(rng[1])))
+    else:
+        raise ValueError("counter_dropout: rng must be (seed, step)")
+    if _hip(x):
+        from . import ext
+        seed, step = (0, 0) if at is not None else rng
+        return ext.require().counter_dropout(x, residual, p, at, seed, step, stream)
+    if at is not None and (at.dtype != torch.int64 or tuple(at.shape) != (2,)
+                           or at.device != x.device):
+        raise ValueError("counter_dropout: rng must be int64 [2] on "
+                         f"{x.device}, got {at.dtype} {tuple(at.shape)} on {at.device}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype
                                  or residual.device != x.device):
         raise ValueError("counter_dropout: residual must have x's shape, dtype and "

@@ -36,80 +36,56 @@ def _gates(g: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
     return torch.sigmoid(gz), torch.sigmoid(-gz), torch.tanh(gn)
 
 
-def _dense(t: Optional[Tensor]) -> Optional[Tensor]:
-    """The kernels step over rows by stride; the last axis has to be dense."""
-    if t is None or t.stride(-1) == 1 or t.shape[-1] == 1:
-        return t
-    return t.contiguous()
-
-
 class _GatedScan(torch.autograd.Function):
+    """Eager form, step by step (the HIP path has its own node)."""
+
     @staticmethod
     def forward(ctx, g: Tensor, h0: Optional[Tensor], mask: Optional[Tensor]):
         ctx.set_materialize_grads(False)
         ctx.h0_dtype = None if h0 is None else h0.dtype
-        g = _dense(g)
-        state = torch.float64 if g.dtype == torch.float64 else torch.float32
-        h0 = None if h0 is None else h0.to(state).contiguous()
-        hip = _hip(g)
-        if hip:
-            from . import ext
-            out, last, *marks = ext.require().gated_scan_fwd(
-                g, h0, mask, any(ctx.needs_input_grad[:2]))
-            marks = marks[0] if marks else None
-        else:
-            z, zc, n = _gates(g)
-            h = (torch.zeros_like(n[:, 0]) if h0 is None else h0)
-            hs = []
-            for t in range(g.shape[1]):
-                new = zc[:, t] * n[:, t] + z[:, t] * h
-                if mask is not None:
-                    new = torch.where(mask[:, t, None] > 0, new, h)
-                h = new
-                hs.append(h)
-            out, last, marks = torch.stack(hs, dim=1).to(g.dtype), h, None
-        ctx.hip = hip
-        ctx.save_for_backward(g, h0, mask, marks)
-        return out, last
+        z, zc, n = _gates(g)
+        h0 = None if h0 is None else h0.to(n.dtype)
+        h = torch.zeros_like(n[:, 0]) if h0 is None else h0
+        hs = []
+        for t in range(g.shape[1]):
+            new = zc[:, t] * n[:, t] + z[:, t] * h
+            if mask is not None:
+                new = torch.where(mask[:, t, None] > 0, new, h)
+            h = new
+            hs.append(h)
+        ctx.save_for_backward(g, h0, mask)
+        return torch.stack(hs, dim=1).to(g.dtype), h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh: Optional[Tensor], dlast: Optional[Tensor]):
-        g, h0, mask, marks = ctx.saved_tensors
+        g, h0, mask = ctx.saved_tensors
         if dh is None and dlast is None:
             return None, None, None
-        if ctx.hip:
-            from . import ext
-            dh = None if dh is None else _dense(dh)
-            dlast = None if dlast is None else dlast.contiguous()
-            dg, *dh0 = ext.require().gated_scan_bwd(g, h0, mask, marks, dh, dlast)
-            dh0 = dh0[0] if dh0 else None
-        else:
-            z, zc, n = _gates(g)
-            h = torch.zeros_like(n[:, 0]) if h0 is None else h0
-            before = []
-            for t in range(g.shape[1]):
-                before.append(h)
-                new = zc[:, t] * n[:, t] + z[:, t] * h
-                if mask is not None:
-                    new = torch.where(mask[:, t, None] > 0, new, h)
-                h = new
-            c = torch.zeros_like(h) if dlast is None else dlast
-            dz, dn = torch.zeros_like(z), torch.zeros_like(n)
-            for t in range(g.shape[1] - 1, -1, -1):
-                if dh is not None:
-                    c = c + _up(dh[:, t])
-                gz = c * (before[t] - n[:, t]) * z[:, t] * zc[:, t]
-                gn = c * zc[:, t] * (1.0 - n[:, t] * n[:, t])
-                new = c * z[:, t]
-                if mask is not None:
-                    on = mask[:, t, None] > 0
-                    gz, gn = torch.where(on, gz, 0.0), torch.where(on, gn, 0.0)
-                    new = torch.where(on, new, c)
-                dz[:, t], dn[:, t], c = gz, gn, new
-            dg, dh0 = torch.cat([dz, dn], dim=-1).to(g.dtype), c
-        dh0 = dh0.to(ctx.h0_dtype) if ctx.h0_dtype is not None else None
-        return dg, dh0, None
+        z, zc, n = _gates(g)
+        h = torch.zeros_like(n[:, 0]) if h0 is None else h0
+        before = []
+        for t in range(g.shape[1]):
+            before.append(h)
+            new = zc[:, t] * n[:, t] + z[:, t] * h
+            if mask is not None:
+                new = torch.where(mask[:, t, None] > 0, new, h)
+            h = new
+        c = torch.zeros_like(h) if dlast is None else dlast
+        dz, dn = torch.zeros_like(z), torch.zeros_like(n)
+        for t in range(g.shape[1] - 1, -1, -1):
+            if dh is not None:
+                c = c + _up(dh[:, t])
+            gz = c * (before[t] - n[:, t]) * z[:, t] * zc[:, t]
+            gn = c * zc[:, t] * (1.0 - n[:, t] * n[:, t])
+            new = c * z[:, t]
+            if mask is not None:
+                on = mask[:, t, None] > 0
+                gz, gn = torch.where(on, gz, 0.0), torch.where(on, gn, 0.0)
+                new = torch.where(on, new, c)
+            dz[:, t], dn[:, t], c = gz, gn, new
+        dg = torch.cat([dz, dn], dim=-1).to(g.dtype)
+        return dg, None if ctx.h0_dtype is None else c.to(ctx.h0_dtype), None
 
 
 def _check_gates(g: Tensor, dim: int, what: str) -> None:
@@ -136,6 +112,9 @@ def gated_scan(g: Tensor, h0: Optional[Tensor] = None,
     mask[B,T] (1 = valid step): a step whose mask is not > 0 leaves the state
     as it is, its gates are not looked at and get a zero gradient; h there is
     the state carried over.  Differentiable in g and h0."""
+    if g.numel() > 0 and _hip(g):
+        from . import ext
+        return ext.require().gated_scan(g, h0, mask)
     _check_gates(g, 3, "gated_scan")
     if h0 is not None:
         _check_state(h0, g, "gated_scan")
@@ -154,16 +133,15 @@ def gated_scan(g: Tensor, h0: Optional[Tensor] = None,
     return _GatedScan.apply(g, h0, mask)
 
 
-@torch.no_grad()
 def gated_step(g: Tensor, h: Tensor) -> Tuple[Tensor, Tensor]:
     """One token of :func:`gated_scan` for decoding: (out[B,D] in g's dtype,
     new state[B,D] f32) from gates g[B,2D] and state h[B,D].  Inference only
     (no autograd); ``h`` is not written."""
+    if g.numel() > 0 and _hip(g):
+        from . import ext
+        return ext.require().gated_step(g, h)
     _check_gates(g, 2, "gated_step")
     _check_state(h, g, "gated_step")
-    if _hip(g) and g.numel() > 0:
-        from . import ext
-        return tuple(ext.require().gated_step(_dense(g), h.float().contiguous()))
-    z, zc, n = _gates(g)
-    new = zc * n + z * h.to(z.dtype)
+    z, zc, n = _gates(g.detach())
+    new = zc * n + z * h.detach().to(z.dtype)
     return new.to(g.dtype), new

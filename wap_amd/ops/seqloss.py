@@ -64,25 +64,17 @@ def _rows_grad(logits: Tensor, e: Tensor, total: Tensor, at: Tensor,
 
 
 class _TokenLogprob(torch.autograd.Function):
+    """Eager form, like the two below (the HIP path has its own nodes)."""
+
     @staticmethod
     def forward(ctx, logits: Tensor, y: Tensor, w: Optional[Tensor]) -> Tensor:
-        ctx.hip = _hip(logits)
-        if ctx.hip:
-            from . import ext
-            logp, stats = ext.require().token_logprob_fwd(logits, y, w)
-            ctx.save_for_backward(logits, y, w, stats)
-            return logp
-        ctx.save_for_backward(logits, y, w, None)
+        ctx.save_for_backward(logits, y, w)
         return _rows(logits, y, w)[0].to(_up(logits).dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dlogp: Tensor):
-        logits, y, w, stats = ctx.saved_tensors
-        if ctx.hip:
-            from . import ext
-            return ext.require().token_logprob_bwd(
-                logits, y, w, stats, dlogp.contiguous()), None, None
+        logits, y, w = ctx.saved_tensors
         _, e, total, at, live = _rows(logits, y, w)
         return _rows_grad(logits, e, total, at, live, dlogp.double()), None, None
 
@@ -106,24 +98,13 @@ class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, y, w, old, adv, ref, lo, hi, beta):
         ctx.set_materialize_grads(False)
-        ctx.hip, ctx.given = _hip(logits), False
-        if ctx.hip:
-            # the gradient of a row needs nothing but the row: it is made
-            # while the row is at hand, for an upstream gradient of one
-            from . import ext
-            grad = ctx.needs_input_grad[0]
-            loss, logp, *rest = ext.require().policy_loss_fwd(
-                logits, y, w, old, adv, ref, lo, hi, beta, grad)
-            if grad:
-                ctx.save_for_backward(logits, y, w, *rest)
-        else:
-            logp, e, total, at, live = _rows(logits, y, w)
-            l, slope = _policy_terms(logp, old, adv, ref, lo, hi, beta)
-            share = w.double() / w.double().sum().clamp_min(1.0)
-            loss = torch.where(live, share * l, 0.0).sum().to(_up(logits).dtype)
-            coef = torch.where(live, share * slope, 0.0)
-            ctx.save_for_backward(logits, y, w, coef)
-            logp = logp.to(_up(logits).dtype)
+        logp, e, total, at, live = _rows(logits, y, w)
+        l, slope = _policy_terms(logp, old, adv, ref, lo, hi, beta)
+        share = w.double() / w.double().sum().clamp_min(1.0)
+        loss = torch.where(live, share * l, 0.0).sum().to(_up(logits).dtype)
+        coef = torch.where(live, share * slope, 0.0)
+        ctx.save_for_backward(logits, y, w, coef)
+        logp = logp.to(_up(logits).dtype)
         ctx.mark_non_differentiable(logp)
         return loss, logp
 
@@ -133,48 +114,29 @@ class _PolicyLoss(torch.autograd.Function):
         none = (None,) * 8
         if up is None:
             return None, *none
-        if not ctx.hip:
-            logits, y, w, coef = ctx.saved_tensors
-            _, e, total, at, live = _rows(logits, y, w)
-            return _rows_grad(logits, e, total, at, live,
-                              coef * up.double()), *none
-        from . import ext
-        logits, y, w, d, stats, coef, held = ctx.saved_tensors
-        if ctx.given:
-            # a second walk over the same graph: the first one's result is the
-            # caller's now, so this one is made anew
-            d, held = torch.empty_like(d), None
-        ctx.given = True
-        ext.require().policy_loss_bwd(logits, y, w, stats, coef, held,
-                                      up.float().contiguous(), d)
-        return d, *none
+        logits, y, w, coef = ctx.saved_tensors
+        _, e, total, at, live = _rows(logits, y, w)
+        return _rows_grad(logits, e, total, at, live, coef * up.double()), *none
 
 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, y, w, ref, beta, eps):
         ctx.set_materialize_grads(False)
-        ctx.hip = _hip(logits)
-        if ctx.hip:
-            from . import ext
-            loss, margin, stats, seq = ext.require().preference_loss_fwd(
-                logits, y, w, ref, beta, eps)
-            ctx.save_for_backward(logits, y, w, stats, seq)
-        else:
-            logp, e, total, at, live = _rows(logits, y, w)
-            gain = torch.where(live, w.double() * (logp - ref.double()), 0.0).sum(1)
-            pairs = logits.shape[0] // 2
-            m = beta * (gain[:pairs] - gain[pairs:])
-            soft = torch.log1p(torch.exp(-m.abs()))
-            loss = ((1 - eps) * (soft + (-m).clamp_min(0))
-                    + eps * (soft + m.clamp_min(0))).mean()
-            slope = beta * (eps * torch.sigmoid(m)
-                            - (1 - eps) * torch.sigmoid(-m)) / pairs
-            dt = _up(logits).dtype
-            loss, margin = loss.to(dt), m.to(dt)
-            ctx.save_for_backward(logits, y, w, torch.cat([slope, -slope]))
+        logp, e, total, at, live = _rows(logits, y, w)
+        gain = torch.where(live, w.double() * (logp - ref.double()), 0.0).sum(1)
+        pairs = logits.shape[0] // 2
+        m = beta * (gain[:pairs] - gain[pairs:])
+        soft = torch.log1p(torch.exp(-m.abs()))
+        loss = ((1 - eps) * (soft + (-m).clamp_min(0))
+                + eps * (soft + m.clamp_min(0))).mean()
+        slope = beta * (eps * torch.sigmoid(m)
+                        - (1 - eps) * torch.sigmoid(-m)) / pairs
+        dt = _up(logits).dtype
+        margin = m.to(dt)
+        ctx.save_for_backward(logits, y, w, torch.cat([slope, -slope]))
         ctx.mark_non_differentiable(margin)
-        return loss, margin
+        return loss.to(dt), margin
 
     @staticmethod
     @once_differentiable
@@ -182,15 +144,10 @@ class _PreferenceLoss(torch.autograd.Function):
         none = (None,) * 5
         if up is None:
             return None, *none
-        if not ctx.hip:
-            logits, y, w, seq = ctx.saved_tensors
-            _, e, total, at, live = _rows(logits, y, w)
-            coef = w.double() * seq.unsqueeze(1) * up.double()
-            return _rows_grad(logits, e, total, at, live, coef), *none
-        from . import ext
-        logits, y, w, stats, seq = ctx.saved_tensors
-        return ext.require().preference_loss_bwd(
-            logits, y, w, stats, seq, up.float().contiguous()), *none
+        logits, y, w, seq = ctx.saved_tensors
+        _, e, total, at, live = _rows(logits, y, w)
+        coef = w.double() * seq.unsqueeze(1) * up.double()
+        return _rows_grad(logits, e, total, at, live, coef), *none
 
 
 def _check(logits: Tensor, y: Tensor, mask: Optional[Tensor], what: str):
@@ -223,6 +180,9 @@ def _per_token(t: Optional[Tensor], logits: Tensor, what: str, name: str):
 def token_logprob(logits: Tensor, y: Tensor, mask: Optional[Tensor] = None) -> Tensor:
     """log p(y)[B,T] (f32) of tokens y[B,T] under logits[B,T,K]; 0 where
     mask[B,T] is 0.  Differentiable in logits."""
+    if logits.numel() > 0 and _hip(logits):
+        from . import ext
+        return ext.require().token_logprob(logits, y, mask)
     logits, y, w = _check(logits, y, mask, "token_logprob")
     if logits.numel() == 0:
         return logits.sum(dim=-1).to(_up(logits).dtype)
@@ -251,12 +211,16 @@ def policy_loss(
     what = "policy_loss"
     if mask is None:
         raise ValueError(f"{what}: mask is required")
-    logits, y, w = _check(logits, y, mask, what)
     if logits.numel() == 0:
         raise ValueError(f"{what}: no tokens: logits are {tuple(logits.shape)}")
     if not (0.0 <= clip_low and 0.0 <= clip_high):
         raise ValueError(f"{what}: clip borders must be >= 0, got "
                          f"{clip_low}, {clip_high}")
+    if _hip(logits):
+        from . import ext
+        return ext.require().policy_loss(logits, y, mask, old_logp, advantage,
+                                         ref_logp, clip_low, clip_high, kl_coef)
+    logits, y, w = _check(logits, y, mask, what)
     if advantage.dim() == 1 and advantage.shape[0] == logits.shape[0]:
         advantage = advantage.unsqueeze(1).expand(logits.shape[:2])
     if tuple(advantage.shape) != tuple(y.shape) or advantage.device != logits.device:
@@ -287,15 +251,19 @@ def preference_loss(
     what = "preference_loss"
     if mask is None:
         raise ValueError(f"{what}: mask is required")
-    logits, y, w = _check(logits, y, mask, what)
+    if ref_logp is None:
+        raise ValueError(f"{what}: ref_logp is required")
     if logits.numel() == 0 or logits.shape[0] % 2:
         raise ValueError(f"{what}: sequences come in pairs: logits are "
                          f"{tuple(logits.shape)}")
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"{what}: label_smoothing must be in [0, 1], got "
                          f"{label_smoothing}")
+    if _hip(logits):
+        from . import ext
+        return ext.require().preference_loss(logits, y, mask, ref_logp, beta,
+                                             label_smoothing)
+    logits, y, w = _check(logits, y, mask, what)
     ref = _per_token(ref_logp, logits, what, "ref_logp")
-    if ref is None:
-        raise ValueError(f"{what}: ref_logp is required")
     return _PreferenceLoss.apply(logits, y, w, ref, float(beta),
                                  float(label_smoothing))
