@@ -39,18 +39,20 @@ struct Gates {
   float z, zc, n;  // z, 1 - z (from the exponential: no cancellation), n
 };
 
-// 2^(x log2 e).  For 16-bit gates one multiplication and the hardware's exp2
-// (relative error |x| 2^-24) are far below the gates' own rounding; f32 gates
-// add what the product lost.
-template <typename T>
+// exp(SCALE x), SCALE a power of two; log2 of it is cut at `most`, which keeps
+// what it is multiplied with finite.  For 16-bit gates one multiplication and
+// the hardware's exp2 (relative error |x| 2^-24) are far below the gates' own
+// rounding; f32 gates add what the product lost.
+template <typename T, int SCALE>
 __device__ __forceinline__ float exp_of(float x, float most) {
-  constexpr float log2e = 1.44269502162933349609375f;
+  constexpr float log2e = SCALE * 1.44269502162933349609375f;
   // the smaller one, NaN if x is NaN
   const float t = __builtin_elementwise_minimum(x * log2e, most);
   const float e = __builtin_amdgcn_exp2f(t);
   if constexpr (sizeof(T) == 4) {
-    // x log2 e - t, with log2 e in two parts; 0 where t is cut or infinite
-    const float lost = fmaf(x, 1.92596299112661746887e-8f, fmaf(x, log2e, -t));
+    // SCALE x log2 e - t, with log2 e in two parts; 0 where t is cut
+    const float lost = fmaf(x, SCALE * 1.92596299112661746887e-8f,
+                            fmaf(x, log2e, -t));
     return fabsf(t) < 120.f ? fmaf(e * 0.693147180559945309f, lost, e) : e;
   }
   return e;
@@ -63,12 +65,12 @@ __device__ __forceinline__ float exp_of(float x, float most) {
 // (5e-8).
 template <typename T>
 __device__ __forceinline__ Gates gates(float gz, float gn) {
-  const float e = exp_of<T>(-gz, 126.f);
+  const float e = exp_of<T, -1>(gz, 126.f);
   Gates r;
   const float z = __builtin_amdgcn_rcpf(1.f + e);
   r.zc = e * z;
   r.z = z - 0x1p-126f;  // nothing but where e was cut: 0
-  const float f = exp_of<T>(2.f * gn, 127.f);
+  const float f = exp_of<T, 2>(gn, 127.f);
   const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + f), 1.f);
   const float q = gn * gn;
   constexpr bool wide = sizeof(T) == 4;
@@ -294,11 +296,31 @@ __device__ __forceinline__ uint32_t steps_on(const Scan& s, long b, long t0,
 }
 
 // A lane's place in a row that is the same in all lanes: the row's address
-// stays scalar work, and the lane's 32-bit byte offset is part of the access.
+// stays in scalar registers, opaque to the compiler, which would otherwise add
+// it up in 64-bit vector work for every access, and the lane's 32-bit byte
+// offset is part of the instruction.
 template <typename T>
-__device__ __forceinline__ T* lane_at(T* row, uint32_t bytes) {
+using Global = __attribute__((address_space(1))) T*;
+
+template <typename V, typename T>
+__device__ __forceinline__ Global<V> lane_at(T* row, uint32_t bytes) {
   typedef std::conditional_t<std::is_const_v<T>, const char, char> byte;
-  return reinterpret_cast<T*>(reinterpret_cast<byte*>(row) + bytes);
+  Global<byte> p = (Global<byte>)row;
+  asm("" : "+s"(p));
+  return (Global<V>)(p + bytes);
+}
+
+// COLD: past the caches, where a pass moves more than the 256 MB of the last
+// one, so that none of it would be there for the next reader (8 x 8192 x 2048
+// bf16: forward 206 us, 217 without, backward 285, 307).  Loads of f32 rows
+// are not: 1 x 50001 x 1000 forward 151 us with cold stores alone, 161 with
+// cold loads too, 158 with neither.
+template <bool COLD, typename V, typename T>
+__device__ __forceinline__ void put(T* row, uint32_t bytes, const V& v) {
+  if constexpr (COLD)
+    __builtin_nontemporal_store(v, lane_at<V>(row, bytes));
+  else
+    *lane_at<V>(row, bytes) = v;
 }
 
 // Rows of a wave, kept as they came (two 16-bit values a register).  Rows past
@@ -306,17 +328,28 @@ __device__ __forceinline__ T* lane_at(T* row, uint32_t bytes) {
 template <typename T, int VEC>
 using Pack = typename VecOf<T, VEC, sizeof(T)>::type;
 
-template <typename T, int VEC, int ROWS>
-__device__ __forceinline__ void load_rows(const T* base, uint32_t bytes,
-                                          long stride, long rows,
-                                          Pack<T, VEC> (&v)[ROWS]) {
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r)
-    v[r] = *reinterpret_cast<const Pack<T, VEC>*>(
-        lane_at(base + (r < rows ? (long)r : rows - 1) * stride, bytes));
+// ROWS + 1 stands for more than ROWS.
+template <int ROWS>
+__device__ __forceinline__ int rows_left(long n) {
+  return n > ROWS ? ROWS + 1 : n < 0 ? 0 : (int)n;
 }
 
-template <typename T, int VEC, int W, int ROWS>
+template <bool COLD, typename T, int VEC, int ROWS>
+__device__ __forceinline__ void load_rows(const T* base, uint32_t bytes,
+                                          long stride, int rows,
+                                          Pack<T, VEC> (&v)[ROWS]) {
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    if constexpr (COLD && sizeof(T) == 2)
+      v[r] = __builtin_nontemporal_load(
+          lane_at<const Pack<T, VEC>>(base, bytes));
+    else
+      v[r] = *lane_at<const Pack<T, VEC>>(base, bytes);
+    if (r + 1 < rows) base += stride;
+  }
+}
+
+template <typename T, int VEC, int W, int ROWS, bool COLD>
 __global__ __launch_bounds__(64 * W) void gscan_fwd_kernel(
     const T* __restrict__ g, Scan s, Chain ch, T* __restrict__ out,
     float* __restrict__ last, float* __restrict__ marks) {
@@ -336,13 +369,13 @@ __global__ __launch_bounds__(64 * W) void gscan_fwd_kernel(
   const uint32_t off = dc * (uint32_t)sizeof(T);
   const long t0 = ((long)at * W + wave) * ROWS;
   const uint32_t on = steps_on<ROWS>(s, b, t0, lane);
-  const long rows = s.L - t0;
+  const int rows = rows_left<ROWS>(s.L - t0);
   float a[ROWS][VEC], x[ROWS][VEC];
   if (on) {
     Pack<T, VEC> rz[ROWS], rn[ROWS];
     const T* p = g + b * s.gsb + t0 * s.gst;
-    load_rows<T, VEC, ROWS>(p, off, s.gst, rows, rz);
-    load_rows<T, VEC, ROWS>(p + s.D, off, s.gst, rows, rn);
+    load_rows<COLD, T, VEC, ROWS>(p, off, s.gst, rows, rz);
+    load_rows<COLD, T, VEC, ROWS>(p + s.D, off, s.gst, rows, rn);
     // all loads leave before the first value is used
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -410,11 +443,11 @@ __global__ __launch_bounds__(64 * W) void gscan_fwd_kernel(
   T* o = out + (b * s.L + t0) * s.D;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    T v[VEC];
+    Pack<T, VEC> v;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) v[j] = (T)fmaf(a[r][j], h[j], x[r][j]);
-    if (r < rows && inside)
-      store_vec<T, VEC>(lane_at(o + (long)r * s.D, off), v);
+    if (r < rows && inside) put<COLD>(o, off, v);
+    o += s.D;
   }
   // steps past the end leave the state as it is
   if (inside && rows > 0 && rows <= ROWS) {
@@ -434,7 +467,7 @@ __global__ __launch_bounds__(64 * W) void gscan_fwd_kernel(
 // are made again from the states that the forward pass left, which reads less
 // than h itself would be, and has them in f32.
 
-template <typename T, int VEC, int W, int ROWS>
+template <typename T, int VEC, int W, int ROWS, bool COLD>
 __global__ __launch_bounds__(64 * W) void gscan_bwd_kernel(
     const T* __restrict__ g, Scan s, Chain ch, const float* __restrict__ marks,
     const T* __restrict__ dh, const float* __restrict__ dlast,
@@ -454,17 +487,17 @@ __global__ __launch_bounds__(64 * W) void gscan_bwd_kernel(
   const uint32_t dc = inside ? d : s.D - VEC;
   const uint32_t off = dc * (uint32_t)sizeof(T);
   const long t0 = ((long)at * W + wave) * ROWS;
-  const long rows = s.L - t0;
+  const int rows = rows_left<ROWS>(s.L - t0);
   const uint32_t on = steps_on<ROWS>(s, b, t0, lane);
   float z[ROWS][VEC], zc[ROWS][VEC], n[ROWS][VEC];
   Pack<T, VEC> ru[ROWS];  // dh stays as it came: half the registers for 16 bits
   if (dh && rows > 0)
-    load_rows<T, VEC, ROWS>(dh + b * s.dsb + t0 * s.dst, off, s.dst, rows, ru);
+    load_rows<COLD, T, VEC, ROWS>(dh + b * s.dsb + t0 * s.dst, off, s.dst, rows, ru);
   if (on) {
     Pack<T, VEC> rz[ROWS], rn[ROWS];
     const T* p = g + b * s.gsb + t0 * s.gst;
-    load_rows<T, VEC, ROWS>(p, off, s.gst, rows, rz);
-    load_rows<T, VEC, ROWS>(p + s.D, off, s.gst, rows, rn);
+    load_rows<COLD, T, VEC, ROWS>(p, off, s.gst, rows, rz);
+    load_rows<COLD, T, VEC, ROWS>(p + s.D, off, s.gst, rows, rn);
     // all loads leave before the first value is used
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -564,7 +597,7 @@ __global__ __launch_bounds__(64 * W) void gscan_bwd_kernel(
       for (int j = 0; j < VEC; ++j)
         c[j] = fmaf(runs[w][lane * VEC + j].x, c[j], back[w][lane * VEC + j]);
   }
-  T* o = dg + (b * s.L + t0) * 2 * s.D;
+  T* o = dg + (b * s.L + t0 + ROWS) * 2 * s.D;
 #pragma unroll
   for (int r = ROWS - 1; r >= 0; --r) {
     float fz[VEC], fn[VEC];
@@ -580,13 +613,13 @@ __global__ __launch_bounds__(64 * W) void gscan_bwd_kernel(
 #pragma unroll
       for (int j = 0; j < VEC; ++j) fz[j] = fn[j] = 0.f;
     }
+    o -= 2 * (long)s.D;
     if (r < rows && inside) {
-      T vz[VEC], vn[VEC];
+      Pack<T, VEC> vz, vn;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) vz[j] = (T)fz[j], vn[j] = (T)fn[j];
-      T* row = o + (long)r * 2 * s.D;
-      store_vec<T, VEC>(lane_at(row, off), vz);
-      store_vec<T, VEC>(lane_at(row + s.D, off), vn);
+      put<COLD>(o, off, vz);
+      put<COLD>(o + s.D, off, vn);
     }
   }
   if (dh0 && inside && t0 == 0) {
@@ -780,15 +813,22 @@ std::vector<torch::Tensor> gated_scan_fwd(
   if (keep && L > (long)back.waves * back.rows)
     marks = torch::empty({B, marks_of(L), D}, last.options());
   const dim3 grid((long)c.ch.groups * c.ch.per * c.ch.tiles);
+  const long moved = 3 * out.numel() * out.element_size();
   by_type(g, "gated_scan", [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     by_shape<T, false>(c.p, [&](auto p) {
       constexpr int V = decltype(p)::vec, W = decltype(p)::waves,
                     R = decltype(p)::rows;
-      hipLaunchKernelGGL((gscan_fwd_kernel<T, V, W, R>), grid,
-                         dim3(64 * W), 0, stream_of(g), data<T>(g), c.s,
-                         c.ch, data<T>(out), data<float>(last),
-                         marks.defined() ? data<float>(marks) : nullptr);
+      auto go = [&](auto cold) {
+        hipLaunchKernelGGL(
+            (gscan_fwd_kernel<T, V, W, R, decltype(cold)::value>), grid,
+            dim3(64 * W), 0, stream_of(g), data<T>(g), c.s, c.ch, data<T>(out), data<float>(last),
+            marks.defined() ? data<float>(marks) : nullptr);
+      };
+      if (moved > (256L << 20))
+        go(std::true_type());
+      else
+        go(std::false_type());
     });
   });
   launched("gated_scan");
@@ -831,17 +871,23 @@ std::vector<torch::Tensor> gated_scan_bwd(
     buf = make_chain(g, &c);
   }
   const dim3 grid((long)c.ch.groups * c.ch.per * c.ch.tiles);
+  const long moved = 5 * (dg.numel() / 2) * dg.element_size();
   by_type(g, "gated_scan", [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     by_shape<T, true>(c.p, [&](auto p) {
       constexpr int V = decltype(p)::vec, W = decltype(p)::waves,
                     R = decltype(p)::rows;
-      hipLaunchKernelGGL((gscan_bwd_kernel<T, V, W, R>), grid,
-                         dim3(64 * W), 0, stream_of(g), data<T>(g), c.s,
-                         c.ch, data_or_null<float>(marks),
-                         data_or_null<T>(dh), data_or_null<float>(dlast),
-                         data<T>(dg),
-                         dh0.defined() ? data<float>(dh0) : nullptr);
+      auto go = [&](auto cold) {
+        hipLaunchKernelGGL(
+            (gscan_bwd_kernel<T, V, W, R, decltype(cold)::value>), grid,
+            dim3(64 * W), 0, stream_of(g), data<T>(g), c.s, c.ch, data_or_null<float>(marks),
+            data_or_null<T>(dh), data_or_null<float>(dlast), data<T>(dg),
+            dh0.defined() ? data<float>(dh0) : nullptr);
+      };
+      if (moved > (256L << 20))
+        go(std::true_type());
+      else
+        go(std::false_type());
     });
   });
   launched("gated_scan backward");
