@@ -18,7 +18,8 @@ valid if any contributing pixel is).
 
 from __future__ import annotations
 
-from typing import Tuple
+import os
+from typing import Optional, Tuple
 
 import torch
 from torch import Tensor, nn
@@ -53,11 +54,37 @@ def downsample_mask(x_mask: Tensor, stride: int) -> Tensor:
     return m.squeeze(1)
 
 
+class _DropoutCounter:
+    """(seed, step) of an encoder's counter-based dropout, on its device.
+
+    The seed is drawn from torch's generator at the first training forward
+    (before any graph capture: a captured step only advances the tensor, so
+    every replay drops anew).  Plain state: it is in no checkpoint, and a
+    resumed run draws a new seed from the restored generator."""
+
+    def __init__(self):
+        self.rng: Optional[Tensor] = None
+
+    def advance(self, device: torch.device) -> None:
+        if self.rng is None or self.rng.device != device:
+            seed = int(torch.randint(1 << 62, ()))
+            self.rng = torch.tensor([seed, 0], dtype=torch.int64, device=device)
+        self.rng[1].add_(1)
+
+
+def _counter_dropout_on() -> bool:
+    """WAP_COUNTER_DROPOUT=1: dropout that stores no mask (opt-in)."""
+    return os.environ.get("WAP_COUNTER_DROPOUT", "0") == "1"
+
+
 class _Bottleneck(nn.Module):
     """BN-ReLU-1x1(4k) -> BN-ReLU-3x3(k), concatenated onto the input."""
 
-    def __init__(self, in_ch: int, growth: int, dropout: float = 0.2):
+    def __init__(self, in_ch: int, growth: int, dropout: float = 0.2,
+                 counter: Optional[_DropoutCounter] = None, stream: int = 0):
         super().__init__()
+        self.counter = counter
+        self.stream = stream
         inter = 4 * growth
         self.bn1 = nn.BatchNorm2d(in_ch)
         self.conv1 = nn.Conv2d(in_ch, inter, 1, bias=False)
@@ -82,7 +109,13 @@ class _Bottleneck(nn.Module):
             out = self.conv1(F.relu(self.bn1(x)))
             out = self.conv2(F.relu(self.bn2(out)))
         if self.dropout > 0 and self.training:
-            out = F.dropout(out, self.dropout)
+            if (self.counter is not None and self.counter.rng is not None
+                    and _counter_dropout_on()):
+                from .. import ops
+                out = ops.counter_dropout(out, self.dropout, self.counter.rng,
+                                          self.stream)
+            else:
+                out = F.dropout(out, self.dropout)
         return torch.cat([x, out], dim=1)
 
 
@@ -116,12 +149,14 @@ class DenseNetEncoder(nn.Module):
         super().__init__()
         self.stem = nn.Conv2d(1, init_ch, 7, stride=2, padding=3, bias=False)
         self.stem_bn = nn.BatchNorm2d(init_ch)
+        self.counter = _DropoutCounter()
         ch = init_ch
         blocks = []
         for b in range(n_blocks):
             layers = []
             for _ in range(layers_per_block):
-                layers.append(_Bottleneck(ch, growth, dropout))
+                layers.append(_Bottleneck(ch, growth, dropout, self.counter,
+                                          b * layers_per_block + len(layers)))
                 ch += growth
             blocks.append(nn.Sequential(*layers))
             if b != n_blocks - 1:
@@ -132,6 +167,8 @@ class DenseNetEncoder(nn.Module):
         self.out_channels = ch  # 684 with defaults
 
     def forward(self, x: Tensor, x_mask: Tensor) -> Tuple[Tensor, Tensor]:
+        if self.training and _counter_dropout_on():
+            self.counter.advance(x.device)
         h = conv_1ch(x, self.stem.weight, stride=2, padding=3)
         if x.is_contiguous(memory_format=torch.channels_last):
             h = h.to(memory_format=torch.channels_last)
