@@ -849,7 +849,7 @@ std::vector<torch::Tensor> gated_scan_bwd(
     TORCH_CHECK(dh->scalar_type() == g.scalar_type() &&
                     dh->device() == g.device() && dh->dim() == 3 &&
                     dh->size(0) == B && dh->size(1) == L &&
-                    dh->size(2) == D && dh->stride(2) == 1,
+                    dh->size(2) == D && (dh->stride(2) == 1 || D == 1),
                 "gated_scan: dh must be [B, T, D] in g's type");
   c10::DeviceGuard guard(g.device());
   auto dg = torch::empty({B, L, 2 * D}, g.options());

@@ -150,13 +150,17 @@ __device__ __forceinline__ void policy_row(
   const double adv = p.adv[(long)(row / T) * p.ab + (long)(row % T) * p.at];
   const double ratio = exp(logp - (double)p.old_logp[row]);
   const double kept = fmin(fmax(ratio, 1.0 - p.lo), 1.0 + p.hi);
-  const double free_ = adv == 0.0 ? 0.0 : ratio * adv, clipped = kept * adv;
+  // an advantage of 0 is worth nothing, however far the ratio is off; a NaN
+  // stays one
+  const double free_ = adv == 0.0 && ratio == ratio ? 0.0 : ratio * adv;
+  const double clipped = kept * adv;
   const bool on = !(free_ > clipped);  // NaN passes through
   *loss = -(on ? free_ : clipped);
   *slope = -(on ? free_ : 0.0);
   if (p.ref) {
     const double gap = (double)p.ref[row] - logp, e = exp(gap);
-    *loss += p.beta * (e - gap - 1.0);
+    // (far out the rest is lost beside e, and infinity less itself is none)
+    *loss += p.beta * (gap > 64.0 ? e : e - gap - 1.0);
     *slope += p.beta * (1.0 - e);
   }
 }
@@ -579,7 +583,7 @@ Rows rows_of(const torch::Tensor& logits, const torch::Tensor& y,
   TORCH_CHECK(logits.dim() == 3 && logits.numel() > 0 &&
                   (logits.stride(2) == 1 || logits.size(2) == 1),
               what, ": logits must be [B, T, K] with a dense last axis");
-  TORCH_CHECK(logits.size(2) < (1 << 30), what, ": too many tokens");
+  TORCH_CHECK(logits.size(2) < (1 << 28), what, ": too many tokens");
   TORCH_CHECK(logits.size(0) * logits.size(1) < (1L << 31), what,
               ": too many rows");
   TORCH_CHECK(y.scalar_type() == at::kLong && y.is_contiguous() &&

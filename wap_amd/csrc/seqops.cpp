@@ -343,6 +343,7 @@ std::tuple<Tensor, Tensor> policy_loss(Tensor logits, Tensor y, Tensor mask,
   OptTensor ref;
   if (ref_logp.has_value())
     ref = per_token(*ref_logp, logits, what, "ref_logp");
+  if (beta == 0.0) ref.reset();  // no term, not 0 times an infinite one
   if (advantage.dim() == 1 && advantage.size(0) == logits.size(0))
     advantage = advantage.unsqueeze(1).expand({logits.size(0), logits.size(1)});
   TORCH_CHECK_VALUE(same_rows(advantage, logits), what,

@@ -111,7 +111,8 @@ def gated_scan(g: Tensor, h0: Optional[Tensor] = None,
 
     mask[B,T] (1 = valid step): a step whose mask is not > 0 leaves the state
     as it is, its gates are not looked at and get a zero gradient; h there is
-    the state carried over.  Differentiable in g and h0."""
+    the state carried over.  A state that is not finite gives infinities or
+    NaN from there on.  Differentiable in g and h0."""
     if g.numel() > 0 and _hip(g):
         from . import ext
         return ext.require().gated_scan(g, h0, mask)

@@ -83,14 +83,17 @@ def _policy_terms(logp, old, adv, ref, lo, hi, beta):
     """(loss, d loss / d logp) of every token, f64."""
     adv = adv.double()
     ratio = torch.exp(logp - old.double())
-    free = torch.where(adv == 0, 0.0, ratio * adv)
+    # an advantage of 0 is worth nothing, however far the ratio is off
+    free = torch.where((adv == 0) & ~ratio.isnan(), 0.0, ratio * adv)
     clipped = ratio.clamp(1.0 - lo, 1.0 + hi) * adv
     on = ~(free > clipped)
     loss, slope = -torch.where(on, free, clipped), -torch.where(on, free, 0.0)
-    if ref is not None:
+    if ref is not None and beta != 0:
         gap = ref.double() - logp
-        loss = loss + beta * (torch.exp(gap) - gap - 1.0)
-        slope = slope + beta * (1.0 - torch.exp(gap))
+        e = torch.exp(gap)
+        # far out the rest is lost beside e, and infinity less itself is none
+        loss = loss + beta * torch.where(gap > 64, e, e - gap - 1.0)
+        slope = slope + beta * (1.0 - e)
     return loss, slope
 
 
@@ -202,7 +205,7 @@ def policy_loss(
         loss = sum(mask * l) / max(sum(mask), 1)
 
     ``advantage`` A is [B,T], or [B] for one value a sequence.  ``old_logp``,
-    ``ref_logp`` (None: no KL term) and A are constants; logp is returned for
+    ``ref_logp`` (None, or kl_coef 0: no KL term) and A are constants; logp is returned for
     monitoring, without a gradient.  Differentiable in logits; where a border
     of the clip is met exactly the unclipped side counts.
 
