@@ -370,8 +370,14 @@ __global__ __launch_bounds__(64 * W) void gscan_fwd_kernel(
   const long t0 = ((long)at * W + wave) * ROWS;
   const uint32_t on = steps_on<ROWS>(s, b, t0, lane);
   const int rows = rows_left<ROWS>(s.L - t0);
+  float h[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j)
+    h[j] = s.h0 && at == 0 ? s.h0[b * s.D + dc + j] : 0.f;
   float a[ROWS][VEC], x[ROWS][VEC];
-  if (on) {
+  // a wave whose steps are all masked reads none of them; short sequences do
+  // not wait for the mask to know
+  if (ch.tiles == 1 ? rows > 0 : on != 0) {
     Pack<T, VEC> rz[ROWS], rn[ROWS];
     const T* p = g + b * s.gsb + t0 * s.gst;
     load_rows<COLD, T, VEC, ROWS>(p, off, s.gst, rows, rz);
@@ -403,10 +409,6 @@ __global__ __launch_bounds__(64 * W) void gscan_fwd_kernel(
       x[r][j] = fmaf(a[r][j], x[r - 1][j], x[r][j]);
       a[r][j] *= a[r - 1][j];
     }
-  float h[VEC];
-#pragma unroll
-  for (int j = 0; j < VEC; ++j)
-    h[j] = s.h0 ? s.h0[b * s.D + dc + j] : 0.f;
   if (W > 1 || ch.tiles > 1) {
     float A[VEC], B[VEC];
 #pragma unroll
@@ -680,19 +682,19 @@ struct Shape {
 // How a pass is cut, by the number of 64-channel blocks and the length (us on
 // an MI355X; "2,8,16": two channels a lane, 8 waves of 16 steps).
 // - Up to 256 steps one tile holds the sequence, and nothing is chained: 16 x
-//   200 x 256 bf16 forward 8.2 in one tile of 1,16,16, 10.0 in two of 2,8,16.
+//   200 x 256 bf16 forward 8.2 in one tile of 1,16,16, 10.7 in two of 1,8,16.
 // - Few blocks: time is the only axis to spread over, and a round trip of the
-//   chain should step far: 1 x 40000 x 128 bf16 forward 28.7 with tiles of 256
-//   steps, 55.2 with 128; from 5 blocks on 128 (2 x 20000 x 512: 42.1, 52.1).
-// - Two channels a lane where that leaves enough workgroups, from 64 blocks:
-//   8 x 8192 x 2048 bf16 forward 194.5, with one 203.7; 8 x 4096 x 256: 21.2,
-//   19.6.  The backward pass then holds 8 steps a wave, to stay under 128
-//   registers: 321.9, with 16 steps of one channel 368.0; 8 x 4096 x 256:
-//   29.3, 27.0.
+//   chain should step far: 1 x 40000 x 128 bf16 forward 28.5 with tiles of 256
+//   steps, 55.6 with 128; from 5 blocks on 128 (2 x 20000 x 512: 48.7, 40.8).
+// - Two channels a lane where that leaves enough workgroups, from 128 blocks:
+//   32 x 4096 x 256 bf16 forward 53.8, with one 65.5; 16 x 200 x 256: 10.2,
+//   8.2; 8 x 4096 x 256: 21.1, 21.7.  The backward pass then holds 8 steps a
+//   wave, to stay under 128 registers: 8 x 8192 x 2048 283, with 16 steps of
+//   one channel 340.
 Shape shape_of(const torch::Tensor& g, bool backward) {
   const long L = g.size(1), D = g.size(2) / 2;
   const long blocks = g.size(0) * ((D + 63) / 64);
-  const bool two = blocks >= 64 && D % 2 == 0 && g.element_size() == 2;
+  const bool two = blocks >= 128 && D % 2 == 0 && g.element_size() == 2;
   const int rows = L <= 8 || (backward && two) ? 8 : 16;
   if (backward && two && L > 64 && L <= 256)  // no room for 16 steps of two
     return {1, L <= 128 ? 8 : 16, 16};

@@ -142,13 +142,24 @@ __device__ __forceinline__ double row_logp(float xy, float m, double sum) {
   return (double)xy - (double)m - log(sum);
 }
 
+// What a row of the policy loss is given, read while the row is on its way.
+struct Given {
+  float adv = 0.f, old_logp = 0.f, ref = 0.f;
+
+  Given() = default;
+  __device__ __forceinline__ Given(const Policy& p, uint32_t row, uint32_t T)
+      : adv(p.adv[(long)(row / T) * p.ab + (long)(row % T) * p.at]),
+        old_logp(p.old_logp[row]),
+        ref(p.ref ? p.ref[row] : 0.f) {}
+};
+
 // Loss of one token and its derivative by logp, both without the 1 / sum of
 // weights.  At a border of the clip the unclipped side counts.
-__device__ __forceinline__ void policy_row(
-    const Policy& p, uint32_t row, uint32_t T, double logp, double* loss,
-    double* slope) {
-  const double adv = p.adv[(long)(row / T) * p.ab + (long)(row % T) * p.at];
-  const double ratio = exp(logp - (double)p.old_logp[row]);
+__device__ __forceinline__ void policy_row(const Policy& p, const Given& g,
+                                           double logp, double* loss,
+                                           double* slope) {
+  const double adv = g.adv;
+  const double ratio = exp(logp - (double)g.old_logp);
   const double kept = fmin(fmax(ratio, 1.0 - p.lo), 1.0 + p.hi);
   // an advantage of 0 is worth nothing, however far the ratio is off; a NaN
   // stays one
@@ -158,7 +169,7 @@ __device__ __forceinline__ void policy_row(
   *loss = -(on ? free_ : clipped);
   *slope = -(on ? free_ : 0.0);
   if (p.ref) {
-    const double gap = (double)p.ref[row] - logp, e = exp(gap);
+    const double gap = (double)g.ref - logp, e = exp(gap);
     // (far out the rest is lost beside e, and infinity less itself is none)
     *loss += p.beta * (gap > 64.0 ? e : e - gap - 1.0);
     *slope += p.beta * (1.0 - e);
@@ -258,7 +269,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
   constexpr int V = Wide<T>::V;
   __shared__ float red_max[NT / 64];
   __shared__ double red_sum[NT / 64];
-  __shared__ float given;
+  __shared__ float row_c;
   const int tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
   // NT = 64: four rows a workgroup, one a wave, no barriers
   const long row = NT == 64 ? (long)blockIdx.x * 4 +
@@ -282,6 +293,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
   }
   const T* x = logits + row_at(r, row);
   const long y = r.y[row];
+  Given given = POLICY ? Given(p, row, r.T) : Given();
   const bool inside = y >= 0 && y < r.K;
   const float xy = inside ? (float)x[y] : NAN;
   const Cut<T> cut(r.K);
@@ -296,6 +308,23 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
     for (int e = 0; e < E; ++e)
       if (e * NT + tid < whole)
         raw[e] = *reinterpret_cast<const vec*>(x + cut.vec_at(e * NT + tid));
+  }
+  // Few rows: every row's first wave adds up the weights by itself, which
+  // spares a launch.
+  double weights = 0.0;
+  if (POLICY && (NT == 64 || threadIdx.x < 64)) {
+    if (count) {
+      weights = *count;
+    } else {
+      double part[4] = {0.0, 0.0, 0.0, 0.0};
+      for (int i = tid; i < r.N; i += 4 * 64)
+#pragma unroll
+        for (int u = 0; u < 4; ++u)  // on their way at once
+          if (i + u * 64 < r.N) part[u] += (double)weight(r, i + u * 64);
+      weights = lanes_sum((part[0] + part[1]) + (part[2] + part[3]));
+    }
+  }
+  if constexpr (E > 0) {
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (e * NT + tid < whole) {
@@ -369,18 +398,9 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
       if (o.stats) o.stats[row] = make_float2(m, s);
     }
     if constexpr (POLICY) {
-      double loss, slope, total;
-      if (count) {
-        total = *count;
-      } else {
-        // few rows: every row's first wave adds up the weights by itself,
-        // which spares a launch
-        total = 0.0;
-        for (long i = tid; i < r.N; i += 64) total += (double)weight(r, i);
-        total = lanes_sum(total);
-      }
-      policy_row(p, row, r.T, logp, &loss, &slope);
-      const double share = (double)w / fmax(total, 1.0);
+      double loss, slope;
+      policy_row(p, given, logp, &loss, &slope);
+      const double share = (double)w / fmax(weights, 1.0);
       c = (float)(share * slope);
       if (tid == 0) {
         o.loss[row] = share * loss;
@@ -391,9 +411,9 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
   if constexpr (POLICY) {
     if (!dlogits) return;
     if constexpr (NT > 64) {
-      if (threadIdx.x == 0) given = c;
+      if (threadIdx.x == 0) row_c = c;
       __syncthreads();
-      c = given;
+      c = row_c;
     }
     const float scale = -c / s;
     T* d = dlogits + row * r.K;
@@ -552,28 +572,53 @@ __global__ void pairs_kernel(const double* __restrict__ gain, long P,
   pairs_loss(gain, P, beta, eps, loss, margin, seq, red);
 }
 
-// Both at once for few tokens: a wave a sequence, up to FEW_SEQS of them.
+// Both at once for few tokens, up to FEW_SEQS sequences: `each` of the 16 waves
+// share one, four tokens of a lane on their way at once.
 constexpr int FEW_SEQS = 256;
 
 __global__ __launch_bounds__(1024) void gain_pairs_kernel(
     const double* __restrict__ logp, const float* __restrict__ ref, Rows r,
-    long P, double beta, double eps, float* __restrict__ loss,
+    long P, int each, double beta, double eps, float* __restrict__ loss,
     float* __restrict__ margin, float* __restrict__ seq) {
   __shared__ double red[16];
-  __shared__ double gain[FEW_SEQS];
-  const int lane = threadIdx.x & 63;
-  for (long b = threadIdx.x >> 6; b < 2 * P; b += 16) {
-    double s = 0.0;
-    for (long t = lane; t < r.T; t += 64) {
-      const long i = b * r.T + t;
-      const float w = weight(r, i);
-      const double got = logp[i], was = (double)ref[i];
-      if (w != 0.f) s += (double)w * (got - was);
+  __shared__ double gain[FEW_SEQS], shares[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int part = wave % each, step = 64 * each, T = (int)r.T;
+  for (int b = wave / each; b < 2 * P; b += 16 / each) {
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int t = part * 64 + lane; t < T; t += 4 * step) {
+      float w[4];
+      double d[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        w[u] = 0.f, d[u] = 0.0;
+        if (t + u * step < T) {
+          const long i = (long)b * T + t + u * step;
+          w[u] = weight(r, i);
+          d[u] = logp[i] - (double)ref[i];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (w[u] != 0.f) s[u] += (double)w[u] * d[u];
     }
-    s = lanes_sum(s);
-    if (lane == 0) gain[b] = s;
+    const double all = lanes_sum((s[0] + s[1]) + (s[2] + s[3]));
+    if (lane == 0) {
+      if (each == 1)
+        gain[b] = all;
+      else
+        shares[wave] = all;  // 2 P * each <= 16: one turn
+    }
   }
   __syncthreads();
+  if (each > 1) {
+    if ((int)threadIdx.x < 2 * P) {
+      double s = 0.0;
+      for (int i = 0; i < each; ++i) s += shares[threadIdx.x * each + i];
+      gain[threadIdx.x] = s;
+    }
+    __syncthreads();
+  }
   pairs_loss(gain, P, beta, eps, loss, margin, seq, red);
 }
 
@@ -819,9 +864,11 @@ std::vector<torch::Tensor> preference_loss_fwd(
                      nullptr);
   // a second launch takes about 5 us; one workgroup reads 16384 tokens in that
   if (r.N <= 16384 && B <= FEW_SEQS) {
+    int each = 1;  // a power of two: 16 waves in whole shares
+    while (2 * each * B <= 16) each *= 2;
     hipLaunchKernelGGL(gain_pairs_kernel, dim3(1), dim3(1024), 0,
                        stream_of(logits), data<double>(logp), data<float>(ref),
-                       r, B / 2, beta, eps, data<float>(loss),
+                       r, B / 2, each, beta, eps, data<float>(loss),
                        data<float>(margin), data<float>(seq));
   } else {
     auto gain = torch::empty({B}, logp.options());
