@@ -705,7 +705,7 @@ void launch_rows(const torch::Tensor& logits, const Rows& r, const Policy& p,
 }
 
 void launch_grad(const torch::Tensor& logits, const Rows& r,
-                 const torch::Tensor& stats, const Factors& f,
+                 const float2* stats, const Factors& f,
                  torch::Tensor& dlogits) {
   by_type(logits, "seqloss", [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
@@ -718,7 +718,7 @@ void launch_grad(const torch::Tensor& logits, const Rows& r,
       hipLaunchKernelGGL((rows_grad_kernel<T, decltype(cold)::value>),
                          dim3(groups, (v + span - 1) / span), dim3(256), 0,
                          stream_of(logits), data<T>(logits), r,
-                         data<float2>(stats), f, lanes, span,
+                         stats, f, lanes, span,
                          data<T>(dlogits));
     });
   });
@@ -752,12 +752,13 @@ torch::Tensor token_logprob_bwd(
   TORCH_CHECK(dlogp.numel() == r.N && stats.numel() == 2 * r.N);
   c10::DeviceGuard guard(logits.device());
   auto d = torch::empty(logits.sizes(), logits.options());
-  launch_grad(logits, r, stats, Factors{data<float>(dlogp)}, d);
+  launch_grad(logits, r, data<float2>(stats), Factors{data<float>(dlogp)}, d);
   return d;
 }
 
-// -> loss, logp and, with `grad`: d logits for an upstream gradient of one,
-// stats, the rows' c, and the factor that each row of d logits holds.
+// -> loss, logp and, with `grad`: d logits for an upstream gradient of one, and
+// of every row its statistics [N, 2], its c [N], and the upstream gradient that
+// its part of d logits holds [N], in one tensor.
 std::vector<torch::Tensor> policy_loss_fwd(
     torch::Tensor logits, torch::Tensor y, torch::Tensor w,
     torch::Tensor old_logp, torch::Tensor adv,
@@ -785,64 +786,57 @@ std::vector<torch::Tensor> policy_loss_fwd(
   auto wide = torch::empty({r.N + 1}, f32.dtype(at::kDouble));
   double* row_loss = data<double>(wide);
   double* count = row_loss + r.N;
-  torch::Tensor dlogits, stats, coef, held;
+  torch::Tensor dlogits, rows;
+  Out o{data<float>(logp), nullptr, nullptr, row_loss, nullptr, nullptr};
   if (grad) {
     dlogits = torch::empty(logits.sizes(), logits.options());
-    stats = torch::empty({r.N, 2}, f32);
-    coef = torch::empty({r.N}, f32);
-    held = torch::empty({r.N}, f32);
+    rows = torch::empty({4 * r.N}, f32);
+    o.stats = data<float2>(rows);
+    o.coef = data<float>(rows) + 2 * r.N;
+    o.held = o.coef + r.N;
   }
   const bool few = r.N <= 1024;
   if (!few)
     hipLaunchKernelGGL((sum_kernel<float, double>), dim3(1), dim3(1024), 0,
                        stream_of(logits), r.w, r.N, count);
-  launch_rows<true>(logits, r, p, few ? nullptr : count,
-                    Out{data<float>(logp), nullptr,
-                        grad ? data<float2>(stats) : nullptr, row_loss,
-                        grad ? data<float>(coef) : nullptr,
-                        grad ? data<float>(held) : nullptr},
+  launch_rows<true>(logits, r, p, few ? nullptr : count, o,
                     grad ? dlogits.data_ptr() : nullptr);
   hipLaunchKernelGGL((sum_kernel<double, float>), dim3(1), dim3(1024), 0,
                      stream_of(logits), row_loss, r.N, data<float>(loss));
   launched("policy_loss");
   if (!grad) return {loss, logp};
-  return {loss, logp, dlogits, stats, coef, held};
+  return {loss, logp, dlogits, rows};
 }
 
-// Brings `dlogits` to the upstream gradient `up`: rows that hold it already
-// (`held`) stay.  Without `held` every row is made.
+// Brings `dlogits` to the upstream gradient `up`: with `again` rows that hold
+// it already stay as they are, without it every row is made.
 void policy_loss_bwd(
-    torch::Tensor logits, torch::Tensor y, torch::Tensor w,
-    torch::Tensor stats, torch::Tensor coef, c10::optional<torch::Tensor> held,
-    torch::Tensor up, torch::Tensor dlogits) {
+    torch::Tensor logits, torch::Tensor y, torch::Tensor w, torch::Tensor rows,
+    bool again, torch::Tensor up, torch::Tensor dlogits) {
   const Rows r = rows_of(logits, y, w, "policy_loss");
-  WAP_F32(stats, logits, "policy_loss");
-  WAP_F32(coef, logits, "policy_loss");
+  WAP_F32(rows, logits, "policy_loss");
   WAP_F32(up, logits, "policy_loss");
-  TORCH_CHECK(up.numel() == 1 && stats.numel() == 2 * r.N &&
-              coef.numel() == r.N && dlogits.is_contiguous() &&
-              dlogits.sizes() == logits.sizes() &&
+  TORCH_CHECK(up.numel() == 1 && rows.numel() == 4 * r.N &&
+              dlogits.is_contiguous() && dlogits.sizes() == logits.sizes() &&
               dlogits.scalar_type() == logits.scalar_type() &&
               dlogits.device() == logits.device());
-  if (held.has_value()) {
-    WAP_F32(*held, logits, "policy_loss");
-    TORCH_CHECK(held->numel() == r.N);
-  }
   c10::DeviceGuard guard(logits.device());
-  const Factors f{data<float>(coef), nullptr, data<float>(up), false};
-  if (!held.has_value()) return launch_grad(logits, r, stats, f, dlogits);
+  const float2* stats = data<float2>(rows);
+  float* coef = data<float>(rows) + 2 * r.N;
+  const Factors f{coef, nullptr, data<float>(up), false};
+  if (!again) return launch_grad(logits, r, stats, f, dlogits);
   const int per = std::min((r.N + 2047) / 2048, 64L);
   by_type(logits, "policy_loss", [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     hipLaunchKernelGGL(rows_again_kernel<T>, dim3((r.N + per - 1) / per),
                        dim3(256), 0, stream_of(logits), data<T>(logits), r,
-                       data<float2>(stats), f, per, data<float>(*held),
-                       data<T>(dlogits));
+                       stats, f, per, coef + r.N, data<T>(dlogits));
   });
   launched("policy_loss gradient");
 }
 
-// -> loss, margins [P], and for the backward pass: stats, d loss / d gain [2P].
+// -> loss, margins [P], and for the backward pass the rows' statistics [N, 2]
+// and the sequences' d loss / d gain [2P] in one tensor.
 std::vector<torch::Tensor> preference_loss_fwd(
     torch::Tensor logits, torch::Tensor y, torch::Tensor w, torch::Tensor ref,
     double beta, double eps) {
@@ -857,10 +851,10 @@ std::vector<torch::Tensor> preference_loss_fwd(
   auto margin = torch::empty({B / 2}, f32);
   // 64-bit: a gain is a small difference of long sums
   auto logp = torch::empty({r.N}, f32.dtype(at::kDouble));
-  auto stats = torch::empty({r.N, 2}, f32);
-  auto seq = torch::empty({B}, f32);
+  auto rows = torch::empty({2 * r.N + B}, f32);
+  float* seq = data<float>(rows) + 2 * r.N;
   launch_rows<false>(logits, r, Policy{}, nullptr,
-                     Out{nullptr, data<double>(logp), data<float2>(stats)},
+                     Out{nullptr, data<double>(logp), data<float2>(rows)},
                      nullptr);
   // a second launch takes about 5 us; one workgroup reads 16384 tokens in that
   if (r.N <= 16384 && B <= FEW_SEQS) {
@@ -869,7 +863,7 @@ std::vector<torch::Tensor> preference_loss_fwd(
     hipLaunchKernelGGL(gain_pairs_kernel, dim3(1), dim3(1024), 0,
                        stream_of(logits), data<double>(logp), data<float>(ref),
                        r, B / 2, each, beta, eps, data<float>(loss),
-                       data<float>(margin), data<float>(seq));
+                       data<float>(margin), seq);
   } else {
     auto gain = torch::empty({B}, logp.options());
     hipLaunchKernelGGL(gain_kernel, dim3(B), dim3(256), 0, stream_of(logits),
@@ -877,24 +871,24 @@ std::vector<torch::Tensor> preference_loss_fwd(
                        data<double>(gain));
     hipLaunchKernelGGL(pairs_kernel, dim3(1), dim3(256), 0, stream_of(logits),
                        data<double>(gain), B / 2, beta, eps, data<float>(loss),
-                       data<float>(margin), data<float>(seq));
+                       data<float>(margin), seq);
   }
   launched("preference_loss");
-  return {loss, margin, stats, seq};
+  return {loss, margin, rows};
 }
 
 torch::Tensor preference_loss_bwd(
-    torch::Tensor logits, torch::Tensor y, torch::Tensor w,
-    torch::Tensor stats, torch::Tensor seq, torch::Tensor up) {
+    torch::Tensor logits, torch::Tensor y, torch::Tensor w, torch::Tensor rows,
+    torch::Tensor up) {
   const Rows r = rows_of(logits, y, w, "preference_loss");
-  WAP_F32(stats, logits, "preference_loss");
-  WAP_F32(seq, logits, "preference_loss");
+  WAP_F32(rows, logits, "preference_loss");
   WAP_F32(up, logits, "preference_loss");
-  TORCH_CHECK(up.numel() == 1 && stats.numel() == 2 * r.N &&
-              seq.numel() == logits.size(0));
+  TORCH_CHECK(up.numel() == 1 && rows.numel() == 2 * r.N + logits.size(0));
   c10::DeviceGuard guard(logits.device());
   auto d = torch::empty(logits.sizes(), logits.options());
-  launch_grad(logits, r, stats,
-              Factors{nullptr, data<float>(seq), data<float>(up), true}, d);
+  launch_grad(logits, r, data<float2>(rows),
+              Factors{nullptr, data<float>(rows) + 2 * r.N, data<float>(up),
+                      true},
+              d);
   return d;
 }

@@ -29,12 +29,12 @@ std::vector<Tensor> policy_loss_fwd(Tensor logits, Tensor y, Tensor w,
                                     Tensor old_logp, Tensor adv, OptTensor ref,
                                     double lo, double hi, double beta,
                                     bool grad);
-void policy_loss_bwd(Tensor logits, Tensor y, Tensor w, Tensor stats,
-                     Tensor coef, OptTensor held, Tensor up, Tensor dlogits);
+void policy_loss_bwd(Tensor logits, Tensor y, Tensor w, Tensor rows, bool again,
+                     Tensor up, Tensor dlogits);
 std::vector<Tensor> preference_loss_fwd(Tensor logits, Tensor y, Tensor w,
                                         Tensor ref, double beta, double eps);
-Tensor preference_loss_bwd(Tensor logits, Tensor y, Tensor w, Tensor stats,
-                           Tensor seq, Tensor up);
+Tensor preference_loss_bwd(Tensor logits, Tensor y, Tensor w, Tensor rows,
+                           Tensor up);
 std::vector<Tensor> counter_dropout_run(Tensor x, OptTensor residual, double p,
                                         OptTensor rng, int64_t seed,
                                         int64_t step, int64_t stream,
@@ -69,6 +69,9 @@ Tensor dense(const Tensor& t) {
 
 // A constant beside the data, in f32.
 Tensor plain(const Tensor& t) {
+  // (each call into the dispatcher that is not made is about 1 us)
+  if (t.scalar_type() == at::kFloat && t.is_contiguous() && !t.requires_grad())
+    return t;
   return t.detach().to(at::kFloat).contiguous();
 }
 
@@ -150,7 +153,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     // row is at hand, for an upstream gradient of one
     auto out = policy_loss_fwd(logits, y, w, old_logp, adv, ref, lo, hi, beta,
                                true);
-    ctx->save_for_backward({logits, y, w, out[2], out[3], out[4], out[5]});
+    ctx->save_for_backward({logits, y, w, out[2], out[3]});
     ctx->saved_data["given"] = false;
     ctx->mark_non_differentiable({out[1]});
     return {out[0], out[1]};
@@ -160,17 +163,12 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     auto s = ctx->get_saved_variables();
     variable_list grads(9);
     if (up[0].defined()) {
-      Tensor d = s[3];
-      OptTensor held = s[6];
-      if (ctx->saved_data["given"].toBool()) {
-        // a second walk over the same graph: the first one's result is the
-        // caller's now, so this one is made anew
-        d = torch::empty_like(d);
-        held.reset();
-      }
+      // in a second walk over the same graph the first one's result is the
+      // caller's, so this one is made anew
+      const bool first = !ctx->saved_data["given"].toBool();
       ctx->saved_data["given"] = true;
-      policy_loss_bwd(s[0], s[1], s[2], s[4], s[5], held, plain(up[0]), d);
-      grads[0] = d;
+      grads[0] = first ? s[3] : torch::empty_like(s[3]);
+      policy_loss_bwd(s[0], s[1], s[2], s[4], first, plain(up[0]), grads[0]);
     }
     return once("policy_loss", std::move(grads));
   }
@@ -181,7 +179,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
                                Tensor w, Tensor ref, double beta, double eps) {
     ctx->set_materialize_grads(false);
     auto out = preference_loss_fwd(logits, y, w, ref, beta, eps);
-    ctx->save_for_backward({logits, y, w, out[2], out[3]});
+    ctx->save_for_backward({logits, y, w, out[2]});
     ctx->mark_non_differentiable({out[1]});
     return {out[0], out[1]};
   }
@@ -190,8 +188,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     auto s = ctx->get_saved_variables();
     variable_list grads(6);
     if (up[0].defined())
-      grads[0] =
-          preference_loss_bwd(s[0], s[1], s[2], s[3], s[4], plain(up[0]));
+      grads[0] = preference_loss_bwd(s[0], s[1], s[2], s[3], plain(up[0]));
     return once("preference_loss", std::move(grads));
   }
 };
@@ -220,7 +217,8 @@ void check_rows(Tensor& logits, Tensor& y, const char* what) {
                     ", ", logits.size(1), "] on ", logits.device(), ", got ",
                     y.sizes(), " on ", y.device());
   logits = dense(logits);
-  y = y.to(at::kLong).contiguous();
+  if (y.scalar_type() != at::kLong || !y.is_contiguous())
+    y = y.to(at::kLong).contiguous();
 }
 
 // ------------------------------------------------------ dropout
@@ -302,9 +300,7 @@ std::tuple<Tensor, Tensor> gated_scan(Tensor g, OptTensor h0, OptTensor mask) {
     TORCH_CHECK_VALUE(same_rows(*mask, g), what, ": mask must be [", g.size(0),
                       ", ", g.size(1), "] on ", g.device(), ", got ",
                       mask->sizes(), " on ", mask->device());
-    mask = (mask->scalar_type() == at::kFloat ? mask->detach()
-                                              : mask->gt(0).to(at::kFloat))
-               .contiguous();
+    mask = plain(mask->scalar_type() == at::kFloat ? *mask : mask->gt(0));
   }
   if (tracked(g) || (h0.has_value() && tracked(*h0))) {
     auto out = GatedScan::apply(g, h0, mask);
@@ -349,7 +345,8 @@ std::tuple<Tensor, Tensor> policy_loss(Tensor logits, Tensor y, Tensor mask,
   TORCH_CHECK_VALUE(same_rows(advantage, logits), what,
                     ": advantage must be [B, T] or [B] on ", logits.device(),
                     ", got ", advantage.sizes(), " on ", advantage.device());
-  advantage = advantage.detach().to(at::kFloat);
+  if (advantage.scalar_type() != at::kFloat || advantage.requires_grad())
+    advantage = advantage.detach().to(at::kFloat);
   if (tracked(logits)) {
     auto out =
         PolicyLoss::apply(logits, y, w, old, advantage, ref, lo, hi, beta);
