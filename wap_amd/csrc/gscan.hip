@@ -16,16 +16,16 @@
 // gates are read once and h is written once: what a chunked scan of two
 // launches reads twice.
 //
-// The chain.  Tile c publishes (A, B) of its steps, waits until the end state
-// of one of the tiles c-1 .. c-WINDOW is there, steps over the tiles between
-// with their (A, B), and publishes its own end state.  The end state is
-// fma(A, state before, B) whichever tile the walk began at, so results do not
-// depend on timing.  Every published word shows by itself whether it has been
-// written (a pattern of ones, a NaN that no result has, stands for "not yet"),
-// so no flag has to be ordered against data; words are read and written with
-// device-scope atomics, since the eight XCDs' L2 caches are not coherent.
-// A tile waits only for tiles of earlier tickets, and a ticket is drawn by a
-// workgroup that is running already: every wait ends.
+// The chain.  A tile publishes (A, B) of its steps, looks at as many tiles
+// before it as it has waves until the end state of one of them is there and
+// the runs of all between, steps over those, and publishes its own end state.
+// The end state is fma(A, state before, B) whichever tile the walk began at, so
+// results do not depend on timing.  Every published word shows by itself
+// whether it has been written (a pattern of ones, a NaN that no result has,
+// stands for "not yet"), so no flag has to be ordered against data; words are
+// read and written with device-scope atomics, since the eight XCDs' L2 caches
+// are not coherent.  A tile waits only for tiles of earlier tickets, and a
+// ticket is drawn by a workgroup that is running already: every wait ends.
 #include <hip/hip_runtime.h>
 
 #include "opcommon.h"
@@ -33,7 +33,6 @@
 namespace {
 
 using namespace wap;
-
 
 struct Gates {
   float z, zc, n;  // z, 1 - z (from the exponential: no cancellation), n
@@ -135,12 +134,16 @@ __device__ __forceinline__ bool next_tile(const Chain& ch, int* block,
   return *block < ch.blocks;
 }
 
+// Tiles of fewer waves hold their whole sequence.
+template <int W>
+constexpr bool may_chain = W >= 8;
+
 // What the waves of a workgroup have seen of the tiles before theirs.
-template <int VEC, int W, int EACH>
+template <int VEC, int W>
 struct Seen {
-  float end[W * EACH][64 * VEC];
-  float2 run[W * EACH][64 * VEC];
-  int has[2][W * EACH];  // 1: the end state, 2: the run; by turns
+  float end[W][64 * VEC];
+  float2 run[W][64 * VEC];
+  int has[2][W];  // 1: the end state, 2: the run; by turns
 };
 
 // A wave's place in the words of tile `at`; tiles are `stride` apart.
@@ -165,72 +168,58 @@ __device__ __forceinline__ void publish(const Chain& ch, int block, int at,
 
 // The whole workgroup finds the state h before tile `at` (tile 0: h as it is)
 // and publishes the state after it; A and B count in wave 0.  Wave w looks at
-// the tiles at-1-w, at-1-w-W, ..: EACH of them, so that a workgroup steps over
-// W EACH tiles in one round trip to memory and holds few registers for it.
-template <int VEC, int W, int EACH>
+// tile at-1-w, so that a workgroup steps over W tiles in one round trip to
+// memory and holds few registers for it.
+template <int VEC, int W>
 __device__ __forceinline__ void walk(const Chain& ch, int block, int at,
                                      int wave, int lane, const float (&A)[VEC],
                                      const float (&B)[VEC],
-                                     Seen<VEC, W, EACH>& seen,
-                                     float (&h)[VEC]) {
+                                     Seen<VEC, W>& seen, float (&h)[VEC]) {
   const long stride = (long)ch.blocks * (64 * VEC);  // from tile to tile
   const long mine = words_at<VEC>(ch, block, at, lane);
   if (at > 0) {
-    const int reach = at < W * EACH ? at : W * EACH;
-    int has[EACH];
-#pragma unroll
-    for (int k = 0; k < EACH; ++k) has[k] = 0;
+    const int reach = at < W ? at : W;
+    const long p = mine - (wave + 1) * stride;  // read where wave < reach
+    int has = 0;
     int from = -1;  // the nearest tile before this one whose end is there
     for (int turn = 0;; turn ^= 1) {
-      // the end first: where it is there the run is not needed, and where it
-      // is not there is time
-      uint32_t e[EACH][VEC];
+      if (wave < reach && !(has & 1)) {
+        // the end first: where it is there the run is not needed, and where it
+        // is not there is time
+        uint32_t e[VEC];
+        bool there = true;
 #pragma unroll
-      for (int k = 0; k < EACH; ++k) {
-        const int i = wave + k * W;
-        if (i < reach && !(has[k] & 1)) {
-          const uint32_t* p = ch.end + mine - (i + 1) * stride;
+        for (int j = 0; j < VEC; ++j) e[j] = peek(ch.end + p + j);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) e[k][j] = peek(p + j);
-        }
-      }
+        for (int j = 0; j < VEC; ++j) there &= e[j] != UNSET;
+        if (__all(there)) {
+          has |= 1;
 #pragma unroll
-      for (int k = 0; k < EACH; ++k) {
-        const int i = wave + k * W;
-        if (i < reach && !(has[k] & 1)) {
-          bool there = true;
+          for (int j = 0; j < VEC; ++j)
+            seen.end[wave][lane * VEC + j] = __uint_as_float(e[j]);
+        } else if (wave + 1 < reach && !(has & 2)) {
+          // (the end of the last tile in reach is not stepped over)
+          uint64_t r[VEC];
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) there &= e[k][j] != UNSET;
+          for (int j = 0; j < VEC; ++j) r[j] = peek(ch.run + p + j);
+          there = true;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) there &= (uint32_t)r[j] != UNSET;
           if (__all(there)) {
-            has[k] |= 1;
+            has |= 2;
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
-              seen.end[i][lane * VEC + j] = __uint_as_float(e[k][j]);
-          } else if (i + 1 < reach && !(has[k] & 2)) {
-            // (the end of the last tile in reach is not stepped over)
-            const uint64_t* p = ch.run + mine - (i + 1) * stride;
-            uint64_t r[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) r[j] = peek(p + j);
-            there = true;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) there &= (uint32_t)r[j] != UNSET;
-            if (__all(there)) {
-              has[k] |= 2;
-#pragma unroll
-              for (int j = 0; j < VEC; ++j)
-                seen.run[i][lane * VEC + j] =
-                    make_float2(__uint_as_float((uint32_t)r[j]),
-                                __uint_as_float((uint32_t)(r[j] >> 32)));
-            }
+              seen.run[wave][lane * VEC + j] =
+                  make_float2(__uint_as_float((uint32_t)r[j]),
+                              __uint_as_float((uint32_t)(r[j] >> 32)));
           }
         }
-        if (lane == 0) seen.has[turn][i] = has[k];
       }
+      if (lane == 0) seen.has[turn][wave] = has;
       __syncthreads();
       // every wave comes to the same answer; the next turn writes elsewhere
 #pragma unroll
-      for (int i = W * EACH - 1; i >= 0; --i) {
+      for (int i = W - 1; i >= 0; --i) {
         const int q = seen.has[turn][i];
         if (i < reach) from = q & 1 ? i : q & 2 ? from : -1;
       }
@@ -354,9 +343,9 @@ __global__ __launch_bounds__(64 * W) void gscan_fwd_kernel(
     const T* __restrict__ g, Scan s, Chain ch, T* __restrict__ out,
     float* __restrict__ last, float* __restrict__ marks) {
   constexpr int CH = 64 * VEC;
-  constexpr int EACH = W < 8 ? 2 : 1;
   __shared__ float2 runs[W][CH];
-  __shared__ Seen<VEC, W, EACH> seen;
+  __shared__ Seen<VEC, may_chain<W> ? W : 1> seen;
+  const bool chained = may_chain<W> && ch.tiles > 1;
   int block, at;
   if (!next_tile(ch, &block, &at)) return;
   const int lane = threadIdx.x & 63;
@@ -377,7 +366,7 @@ __global__ __launch_bounds__(64 * W) void gscan_fwd_kernel(
   float a[ROWS][VEC], x[ROWS][VEC];
   // a wave whose steps are all masked reads none of them; short sequences do
   // not wait for the mask to know
-  if (ch.tiles == 1 ? rows > 0 : on != 0) {
+  if (chained ? on != 0 : rows > 0) {
     Pack<T, VEC> rz[ROWS], rn[ROWS];
     const T* p = g + b * s.gsb + t0 * s.gst;
     load_rows<COLD, T, VEC, ROWS>(p, off, s.gst, rows, rz);
@@ -409,7 +398,7 @@ __global__ __launch_bounds__(64 * W) void gscan_fwd_kernel(
       x[r][j] = fmaf(a[r][j], x[r - 1][j], x[r][j]);
       a[r][j] *= a[r - 1][j];
     }
-  if (W > 1 || ch.tiles > 1) {
+  if constexpr (W > 1) {
     float A[VEC], B[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
@@ -417,7 +406,7 @@ __global__ __launch_bounds__(64 * W) void gscan_fwd_kernel(
       runs[wave][lane * VEC + j] = make_float2(A[j], B[j]);
     }
     __syncthreads();
-    if (ch.tiles > 1) {
+    if (chained) {
       if (wave == 0) {
         for (int w = 1; w < W; ++w)
 #pragma unroll
@@ -428,7 +417,8 @@ __global__ __launch_bounds__(64 * W) void gscan_fwd_kernel(
           }
         publish<VEC>(ch, block, at, lane, A, B);
       }
-      walk<VEC, W, EACH>(ch, block, at, wave, lane, A, B, seen, h);
+      if constexpr (may_chain<W>)
+        walk<VEC, W>(ch, block, at, wave, lane, A, B, seen, h);
     }
     for (int w = 0; w < wave; ++w)
 #pragma unroll
@@ -474,10 +464,11 @@ __global__ __launch_bounds__(64 * W) void gscan_bwd_kernel(
     const T* __restrict__ g, Scan s, Chain ch, const float* __restrict__ marks,
     const T* __restrict__ dh, const float* __restrict__ dlast,
     T* __restrict__ dg, float* __restrict__ dh0) {
-  constexpr int CH = 64 * VEC, EACH = W < 8 ? 2 : 1;
+  constexpr int CH = 64 * VEC;
   __shared__ float2 runs[W][CH];
   __shared__ float back[W][CH];
-  __shared__ Seen<VEC, W, EACH> seen;
+  __shared__ Seen<VEC, may_chain<W> ? W : 1> seen;
+  const bool chained = may_chain<W> && ch.tiles > 1;
   int block, from_end;
   if (!next_tile(ch, &block, &from_end)) return;
   const int at = ch.tiles - 1 - from_end;
@@ -494,7 +485,8 @@ __global__ __launch_bounds__(64 * W) void gscan_bwd_kernel(
   float z[ROWS][VEC], zc[ROWS][VEC], n[ROWS][VEC];
   Pack<T, VEC> ru[ROWS];  // dh stays as it came: half the registers for 16 bits
   if (dh && rows > 0)
-    load_rows<COLD, T, VEC, ROWS>(dh + b * s.dsb + t0 * s.dst, off, s.dst, rows, ru);
+    load_rows<COLD, T, VEC, ROWS>(dh + b * s.dsb + t0 * s.dst, off, s.dst, rows,
+                                  ru);
   if (on) {
     Pack<T, VEC> rz[ROWS], rn[ROWS];
     const T* p = g + b * s.gsb + t0 * s.gst;
@@ -539,7 +531,7 @@ __global__ __launch_bounds__(64 * W) void gscan_bwd_kernel(
     c[j] = dlast ? dlast[b * s.D + dc + j] : 0.f;
   }
   float A[VEC], C[VEC];
-  if (W > 1 || ch.tiles > 1) {
+  if constexpr (W > 1) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       float B = 0.f;
@@ -556,7 +548,7 @@ __global__ __launch_bounds__(64 * W) void gscan_bwd_kernel(
       back[wave][lane * VEC + j] = C[j];
     }
     __syncthreads();
-    if (ch.tiles > 1) {
+    if (chained) {
       if (wave == 0) {
         // the waves' runs from the end; this one's own is the last
 #pragma unroll
@@ -570,8 +562,8 @@ __global__ __launch_bounds__(64 * W) void gscan_bwd_kernel(
           C[j] = fmaf(A[j], b, C[j]);
           A[j] *= a;
         }
+        publish<VEC>(ch, block, from_end, lane, A, C);
       }
-      if (wave == 0) publish<VEC>(ch, block, from_end, lane, A, C);
     }
     for (int w = 0; w < wave; ++w)
 #pragma unroll
@@ -591,9 +583,10 @@ __global__ __launch_bounds__(64 * W) void gscan_bwd_kernel(
       zc[r][j] = q * z[r][j] * (past - m);
       n[r][j] = q * fmaf(-m, m, 1.f);
     }
-  if (W > 1 || ch.tiles > 1) {
-    if (ch.tiles > 1)
-      walk<VEC, W, EACH>(ch, block, from_end, wave, lane, A, C, seen, c);
+  if constexpr (W > 1) {
+    if constexpr (may_chain<W>)
+      if (chained)
+        walk<VEC, W>(ch, block, from_end, wave, lane, A, C, seen, c);
     for (int w = W - 1; w > wave; --w)
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
@@ -731,6 +724,7 @@ Cut cut_of(const torch::Tensor& g, const c10::optional<torch::Tensor>& h0,
   const long tiles = (c.s.L + step - 1) / step;
   TORCH_CHECK(blocks < (1L << 30) && tiles < (1L << 30),
               "gated_scan: too many sequences, channels or steps");
+  TORCH_CHECK(tiles == 1 || c.p.waves >= 8, "gated_scan: no such shape");
   c.ch.blocks = blocks;
   c.ch.tiles = tiles;
   c.ch.groups = tiles == 1 ? 1 : std::min(blocks, 64L);
@@ -882,8 +876,8 @@ std::vector<torch::Tensor> gated_scan_bwd(
       auto go = [&](auto cold) {
         hipLaunchKernelGGL(
             (gscan_bwd_kernel<T, V, W, R, decltype(cold)::value>), grid,
-            dim3(64 * W), 0, stream_of(g), data<T>(g), c.s, c.ch, data_or_null<float>(marks),
-            data_or_null<T>(dh), data_or_null<float>(dlast), data<T>(dg),
+            dim3(64 * W), 0, stream_of(g), data<T>(g), c.s, c.ch,
+            data_or_null<float>(marks), data_or_null<T>(dh), data_or_null<float>(dlast), data<T>(dg),
             dh0.defined() ? data<float>(dh0) : nullptr);
       };
       if (moved > (256L << 20))

@@ -20,23 +20,6 @@ struct VecOf {
   typedef T type __attribute__((ext_vector_type(N), aligned(A)));
 };
 
-template <typename T, int N, int A = sizeof(T)>
-__device__ __forceinline__ void load_vec(const T* p, T (&r)[N]) {
-  typedef typename VecOf<T, N, A>::type V;
-  const V v = *reinterpret_cast<const V*>(p);
-#pragma unroll
-  for (int i = 0; i < N; ++i) r[i] = v[i];
-}
-
-template <typename T, int N, int A = sizeof(T)>
-__device__ __forceinline__ void store_vec(T* p, const T (&r)[N]) {
-  typedef typename VecOf<T, N, A>::type V;
-  V v;
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = r[i];
-  *reinterpret_cast<V*>(p) = v;
-}
-
 // Sum / maximum over the 64 lanes, the result on every lane.
 template <typename F>
 __device__ __forceinline__ F lanes_sum(F v) {
