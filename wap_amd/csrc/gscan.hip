@@ -38,18 +38,19 @@ struct Gates {
   float z, zc, n;  // z, 1 - z (from the exponential: no cancellation), n
 };
 
-// exp(SCALE x), SCALE a power of two; log2 of it is cut at `most`, which keeps
-// what it is multiplied with finite.  For 16-bit gates one multiplication and
-// the hardware's exp2 (relative error |x| 2^-24) are far below the gates' own
+// exp(SCALE x), SCALE a power of two; with CUT at most 2^126, which keeps what
+// it is multiplied with finite.  For 16-bit gates one multiplication and the
+// hardware's exp2 (relative error |x| 2^-24) are far below the gates' own
 // rounding; f32 gates add what the product lost.
-template <typename T, int SCALE>
-__device__ __forceinline__ float exp_of(float x, float most) {
+template <typename T, int SCALE, bool CUT>
+__device__ __forceinline__ float exp_of(float x) {
   constexpr float log2e = SCALE * 1.44269502162933349609375f;
+  float t = x * log2e;
   // the smaller one, NaN if x is NaN
-  const float t = __builtin_elementwise_minimum(x * log2e, most);
+  if constexpr (CUT) t = __builtin_elementwise_minimum(t, 126.f);
   const float e = __builtin_amdgcn_exp2f(t);
   if constexpr (sizeof(T) == 4) {
-    // SCALE x log2 e - t, with log2 e in two parts; 0 where t is cut
+    // SCALE x log2 e - t, with log2 e in two parts; not where t is cut or e ends
     const float lost = fmaf(x, SCALE * 1.92596299112661746887e-8f,
                             fmaf(x, log2e, -t));
     return fabsf(t) < 120.f ? fmaf(e * 0.693147180559945309f, lost, e) : e;
@@ -64,12 +65,12 @@ __device__ __forceinline__ float exp_of(float x, float most) {
 // (5e-8).
 template <typename T>
 __device__ __forceinline__ Gates gates(float gz, float gn) {
-  const float e = exp_of<T, -1>(gz, 126.f);
+  const float e = exp_of<T, -1, true>(gz);
   Gates r;
   const float z = __builtin_amdgcn_rcpf(1.f + e);
   r.zc = e * z;
   r.z = z - 0x1p-126f;  // nothing but where e was cut: 0
-  const float f = exp_of<T, 2>(gn, 127.f);
+  const float f = exp_of<T, 2, false>(gn);
   const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + f), 1.f);
   const float q = gn * gn;
   constexpr bool wide = sizeof(T) == 4;
