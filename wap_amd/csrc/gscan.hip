@@ -115,8 +115,10 @@ __device__ __forceinline__ void post(W* p, W v) {
 // The next tile of this workgroup's group, in time order over all channel
 // blocks of the group: (block, place in time). False: none.
 // The grid has groups * per * tiles workgroups and blockIdx % groups is the
-// group, so that with workgroups dealt to the XCDs in turn a chain stays on
-// one XCD.
+// group, so that with workgroups dealt to the eight XCDs in turn a chain stays
+// on one XCD.  Groups of one XCD take blocks side by side: where rows are no
+// multiple of a cache line, the lines that two blocks share then come from one
+// L2.
 __device__ __forceinline__ bool next_tile(const Chain& ch, int* block,
                                           int* at) {
   const int grp = blockIdx.x % ch.groups;
@@ -131,7 +133,10 @@ __device__ __forceinline__ bool next_tile(const Chain& ch, int* block,
     k = __builtin_amdgcn_readfirstlane(drawn);
   }
   *at = k / ch.per;
-  *block = k % ch.per * ch.groups + grp;
+  // (4 x 8000 x 1001 f32 forward 99.5 us, 108 in the groups' own order)
+  const int side =
+      ch.groups % 8 ? grp : grp % 8 * (ch.groups / 8) + grp / 8;
+  *block = k % ch.per * ch.groups + side;
   return *block < ch.blocks;
 }
 
@@ -302,9 +307,9 @@ __device__ __forceinline__ Global<V> lane_at(T* row, uint32_t bytes) {
 
 // COLD: past the caches, where a pass moves more than the 256 MB of the last
 // one, so that none of it would be there for the next reader (8 x 8192 x 2048
-// bf16: forward 206 us, 217 without, backward 285, 307).  Loads of f32 rows
-// are not: 1 x 50001 x 1000 forward 151 us with cold stores alone, 161 with
-// cold loads too, 158 with neither.
+// bf16: forward 206 us, 217 without, backward 285, 307).  Not where channel
+// blocks share cache lines: the caches put those together (4 x 8000 x 1001
+// f32: forward 92.5 us, with cold stores 99.5, with cold loads too 108).
 template <bool COLD, typename V, typename T>
 __device__ __forceinline__ void put(T* row, uint32_t bytes, const V& v) {
   if constexpr (COLD)
@@ -330,7 +335,7 @@ __device__ __forceinline__ void load_rows(const T* base, uint32_t bytes,
                                           Pack<T, VEC> (&v)[ROWS]) {
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    if constexpr (COLD && sizeof(T) == 2)
+    if constexpr (COLD)
       v[r] = __builtin_nontemporal_load(
           lane_at<const Pack<T, VEC>>(base, bytes));
     else
@@ -680,15 +685,17 @@ struct Shape {
 // - Few blocks: time is the only axis to spread over, and a round trip of the
 //   chain should step far: 1 x 40000 x 128 bf16 forward 28.5 with tiles of 256
 //   steps, 55.6 with 128; from 5 blocks on 128 (2 x 20000 x 512: 48.7, 40.8).
-// - Two channels a lane where that leaves enough workgroups, from 128 blocks:
-//   32 x 4096 x 256 bf16 forward 53.8, with one 65.5; 16 x 200 x 256: 10.2,
-//   8.2; 8 x 4096 x 256: 21.1, 21.7.  The backward pass then holds 8 steps a
-//   wave, to stay under 128 registers: 8 x 8192 x 2048 283, with 16 steps of
-//   one channel 340.
+// - Two channels a lane where that leaves enough workgroups, from 64 blocks on
+//   (short sequences, all latency, from 128): 32 x 4096 x 256 bf16 forward
+//   53.8, with one 65.5; 4 x 8192 x 1500: 87, 135; 8 x 4096 x 256: 21.1, 21.7;
+//   16 x 200 x 256: 10.2, 8.2.  The backward pass then holds 8 steps a wave, to
+//   stay under 128 registers: 8 x 8192 x 2048 283, with 16 steps of one channel
+//   340.
 Shape shape_of(const torch::Tensor& g, bool backward) {
   const long L = g.size(1), D = g.size(2) / 2;
   const long blocks = g.size(0) * ((D + 63) / 64);
-  const bool two = blocks >= 128 && D % 2 == 0 && g.element_size() == 2;
+  const bool two = blocks >= (L > 256 ? 64 : 128) && D % 2 == 0 &&
+                   g.element_size() == 2;
   const int rows = L <= 8 || (backward && two) ? 8 : 16;
   if (backward && two && L > 64 && L <= 256)  // no room for 16 steps of two
     return {1, L <= 128 ? 8 : 16, 16};
@@ -757,6 +764,13 @@ torch::Tensor make_chain(const torch::Tensor& g, Cut* c) {
   return buf;
 }
 
+// Whether channel blocks share no cache line.
+bool in_lines(const torch::Tensor& t, long D) {
+  const long line = 128 / t.element_size();
+  return D % line == 0 && t.stride(0) % line == 0 && t.stride(1) % line == 0 &&
+         reinterpret_cast<uintptr_t>(t.data_ptr()) % 128 == 0;
+}
+
 template <int VEC, int W, int ROWS>
 struct Fixed {
   static constexpr int vec = VEC, waves = W, rows = ROWS;
@@ -810,19 +824,20 @@ std::vector<torch::Tensor> gated_scan_fwd(
   if (keep && L > (long)back.waves * back.rows)
     marks = torch::empty({B, marks_of(L), D}, last.options());
   const dim3 grid((long)c.ch.groups * c.ch.per * c.ch.tiles);
-  const long moved = 3 * out.numel() * out.element_size();
+  const bool cold =
+      3 * out.numel() * out.element_size() > (256L << 20) && in_lines(g, D);
   by_type(g, "gated_scan", [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     by_shape<T, false>(c.p, [&](auto p) {
       constexpr int V = decltype(p)::vec, W = decltype(p)::waves,
                     R = decltype(p)::rows;
-      auto go = [&](auto cold) {
+      auto go = [&](auto past) {
         hipLaunchKernelGGL(
-            (gscan_fwd_kernel<T, V, W, R, decltype(cold)::value>), grid,
+            (gscan_fwd_kernel<T, V, W, R, decltype(past)::value>), grid,
             dim3(64 * W), 0, stream_of(g), data<T>(g), c.s, c.ch, data<T>(out), data<float>(last),
             marks.defined() ? data<float>(marks) : nullptr);
       };
-      if (moved > (256L << 20))
+      if (cold)
         go(std::true_type());
       else
         go(std::false_type());
@@ -868,20 +883,22 @@ std::vector<torch::Tensor> gated_scan_bwd(
     buf = make_chain(g, &c);
   }
   const dim3 grid((long)c.ch.groups * c.ch.per * c.ch.tiles);
-  const long moved = 5 * (dg.numel() / 2) * dg.element_size();
+  const bool cold =
+      5 * (dg.numel() / 2) * dg.element_size() > (256L << 20) &&
+      in_lines(g, D) && (!dh.has_value() || in_lines(*dh, D));
   by_type(g, "gated_scan", [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     by_shape<T, true>(c.p, [&](auto p) {
       constexpr int V = decltype(p)::vec, W = decltype(p)::waves,
                     R = decltype(p)::rows;
-      auto go = [&](auto cold) {
+      auto go = [&](auto past) {
         hipLaunchKernelGGL(
-            (gscan_bwd_kernel<T, V, W, R, decltype(cold)::value>), grid,
+            (gscan_bwd_kernel<T, V, W, R, decltype(past)::value>), grid,
             dim3(64 * W), 0, stream_of(g), data<T>(g), c.s, c.ch,
             data_or_null<float>(marks), data_or_null<T>(dh), data_or_null<float>(dlast), data<T>(dg),
             dh0.defined() ? data<float>(dh0) : nullptr);
       };
-      if (moved > (256L << 20))
+      if (cold)
         go(std::true_type());
       else
         go(std::false_type());
