@@ -259,8 +259,8 @@ __device__ __forceinline__ void zero_span(T* d, int K, int begin, int end,
 // NT threads a row.  E > 0: the row waits in registers, E 16-byte vectors a
 // thread, packed as they came.  E = 0: rows too long for that are read once
 // for the sums (a running maximum and sum a thread) and again for the
-// gradient.  Bound by memory: 18 instruction slots an element of bf16 are 0.4
-// of what reading and writing it takes.
+// gradient.  Bound by memory: about 20 instruction slots an element of bf16 are
+// half of what reading and writing it takes.
 template <typename T, int NT, int E, bool POLICY, bool COLD>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
     const T* __restrict__ logits, Rows r, Policy p,
@@ -309,7 +309,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
       if (e * NT + tid < whole)
         raw[e] = *reinterpret_cast<const vec*>(x + cut.vec_at(e * NT + tid));
   }
-  // Few rows: every row's first wave adds up the weights by itself, which
+  // Up to 1024 rows every row adds up the weights by itself, which
   // spares a launch.
   double weights = 0.0;
   if (POLICY && (NT == 64 || threadIdx.x < 64)) {
