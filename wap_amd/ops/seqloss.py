@@ -210,7 +210,9 @@ def policy_loss(
     of the clip is met exactly the unclipped side counts.
 
     Memory: with a gradient wanted, the call keeps a second tensor of the size
-    of logits (their gradient) until the backward pass."""
+    of logits (their gradient) until the backward pass.  A backward pass that
+    is captured apart from its forward pass may be replayed alone as long as
+    nothing else has written into the gradient that it returned."""
     what = "policy_loss"
     if mask is None:
         raise ValueError(f"{what}: mask is required")
