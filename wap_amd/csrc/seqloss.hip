@@ -552,7 +552,10 @@ __device__ __forceinline__ void pairs_loss(const double* gain, long P,
   for (long i = threadIdx.x; i < P; i += blockDim.x) {
     const double m = beta * (gain[i] - gain[P + i]);
     const double e = exp(-fabs(m)), soft = log1p(e), big = 1.0 / (1.0 + e);
-    s += (1.0 - eps) * (soft + fmax(-m, 0.0)) + eps * (soft + fmax(m, 0.0));
+    // a term of coefficient 0 is none, not 0 times an infinite one: the margin
+    // is infinite where a token has been ruled out
+    if (eps < 1.0) s += (1.0 - eps) * (soft + fmax(-m, 0.0));
+    if (eps > 0.0) s += eps * (soft + fmax(m, 0.0));
     // sigmoid(m), sigmoid(-m) from the one exponential
     const double up = m >= 0.0 ? big : e * big, down = m >= 0.0 ? e * big : big;
     const double d = beta * (eps * up - (1.0 - eps) * down) / (double)P;

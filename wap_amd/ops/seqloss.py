@@ -131,8 +131,14 @@ class _PreferenceLoss(torch.autograd.Function):
         pairs = logits.shape[0] // 2
         m = beta * (gain[:pairs] - gain[pairs:])
         soft = torch.log1p(torch.exp(-m.abs()))
-        loss = ((1 - eps) * (soft + (-m).clamp_min(0))
-                + eps * (soft + m.clamp_min(0))).mean()
+        # a term of coefficient 0 is none, not 0 times an infinite one: the
+        # margin is infinite where a token has been ruled out
+        each = torch.zeros_like(m)
+        if eps < 1:
+            each = each + (1 - eps) * (soft + (-m).clamp_min(0))
+        if eps > 0:
+            each = each + eps * (soft + m.clamp_min(0))
+        loss = each.mean()
         slope = beta * (eps * torch.sigmoid(m)
                         - (1 - eps) * torch.sigmoid(-m)) / pairs
         dt = _up(logits).dtype
@@ -252,7 +258,10 @@ def preference_loss(
                            - s log sigmoid(-margin_i) ),  s = label_smoothing
 
     ``ref_logp`` [2P,T] is the reference's ``token_logprob``, a constant; the
-    margin is returned without a gradient.  Differentiable in logits."""
+    margin is returned without a gradient.  Differentiable in logits.  A token
+    of probability 0 makes its pair's margin infinite and the loss what the
+    formula tends to: nothing of that pair where the token is rejected and s
+    is 0."""
     what = "preference_loss"
     if mask is None:
         raise ValueError(f"{what}: mask is required")
