@@ -759,6 +759,18 @@ torch::Tensor token_logprob_bwd(
   return d;
 }
 
+// Which capture the current stream of `like`'s device belongs to; 0: none.
+int64_t capture_of(const torch::Tensor& like) {
+  hipStreamCaptureStatus status;
+  unsigned long long id = 0;
+  const hipError_t err = hipStreamGetCaptureInfo(stream_of(like), &status, &id);
+  if (err != hipSuccess) {
+    (void)hipGetLastError();  // told here, not by the next launch
+    TORCH_CHECK(false, "policy_loss: ", hipGetErrorString(err));
+  }
+  return status == hipStreamCaptureStatusNone ? 0 : (int64_t)id + 1;
+}
+
 // -> loss, logp and, with `grad`: d logits for an upstream gradient of one, and
 // of every row its statistics [N, 2], its c [N], and the upstream gradient that
 // its part of d logits holds [N], in one tensor.

@@ -31,6 +31,7 @@ std::vector<Tensor> policy_loss_fwd(Tensor logits, Tensor y, Tensor w,
                                     bool grad);
 void policy_loss_bwd(Tensor logits, Tensor y, Tensor w, Tensor rows, bool again,
                      Tensor up, Tensor dlogits);
+int64_t capture_of(const Tensor& like);
 std::vector<Tensor> preference_loss_fwd(Tensor logits, Tensor y, Tensor w,
                                         Tensor ref, double beta, double eps);
 Tensor preference_loss_bwd(Tensor logits, Tensor y, Tensor w, Tensor rows,
@@ -153,8 +154,11 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     // row is at hand, for an upstream gradient of one
     auto out = policy_loss_fwd(logits, y, w, old_logp, adv, ref, lo, hi, beta,
                                true);
-    ctx->save_for_backward({logits, y, w, out[2], out[3]});
-    ctx->saved_data["given"] = false;
+    ctx->save_for_backward({logits, y, w, out[3]});
+    // not among the saved tensors: it is handed out, and from then on the
+    // caller's to write into
+    ctx->saved_data["made"] = out[2];
+    ctx->saved_data["capture"] = capture_of(logits);
     ctx->mark_non_differentiable({out[1]});
     return {out[0], out[1]};
   }
@@ -163,12 +167,22 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     auto s = ctx->get_saved_variables();
     variable_list grads(9);
     if (up[0].defined()) {
-      // in a second walk over the same graph the first one's result is the
-      // caller's, so this one is made anew
-      const bool first = !ctx->saved_data["given"].toBool();
-      ctx->saved_data["given"] = true;
-      grads[0] = first ? s[3] : torch::empty_like(s[3]);
-      policy_loss_bwd(s[0], s[1], s[2], s[4], first, plain(up[0]), grads[0]);
+      // Handed out once, and only where the forward pass runs whenever this
+      // pass does: eagerly, or in the same captured graph.  A pass that is
+      // replayed without the forward pass would find what the caller has
+      // written there, and a forward pass that is replayed without this one
+      // would write into what the caller was given.  Any other walk makes the
+      // gradient anew.
+      auto made = ctx->saved_data.find("made");
+      const bool take = made != ctx->saved_data.end() &&
+                        ctx->saved_data["capture"].toInt() == capture_of(s[0]);
+      if (take) {
+        grads[0] = made->second.toTensor();
+        ctx->saved_data.erase(made);
+      } else {
+        grads[0] = torch::empty(s[0].sizes(), s[0].options());
+      }
+      policy_loss_bwd(s[0], s[1], s[2], s[3], take, plain(up[0]), grads[0]);
     }
     return once("policy_loss", std::move(grads));
   }

@@ -216,9 +216,10 @@ def policy_loss(
     of the clip is met exactly the unclipped side counts.
 
     Memory: with a gradient wanted, the call keeps a second tensor of the size
-    of logits (their gradient) until the backward pass.  A backward pass that
-    is captured apart from its forward pass may be replayed alone as long as
-    nothing else has written into the gradient that it returned."""
+    of logits (their gradient for an upstream gradient of one) until the
+    backward pass.  Another upstream gradient, a second walk over a kept graph
+    and a backward pass captured apart from its forward pass read the logits
+    and write the gradient once more."""
     what = "policy_loss"
     if mask is None:
         raise ValueError(f"{what}: mask is required")
