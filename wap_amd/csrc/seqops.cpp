@@ -43,8 +43,17 @@ std::vector<Tensor> counter_dropout_run(Tensor x, OptTensor residual, double p,
 
 namespace {
 
-bool tracked(const Tensor& t) {
+// Whether a gradient is wanted by t.  A tangent, which no kernel here carries
+// on, is refused: without it the output would read as a zero derivative.
+bool tracked(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), what,
+                              " has no forward-mode derivative");
   return at::GradMode::is_enabled() && t.requires_grad();
+}
+
+bool tracked(const Tensor& t, const OptTensor& u, const char* what) {
+  const bool second = u.has_value() && tracked(*u, what);
+  return tracked(t, what) || second;
 }
 
 OptTensor given(const Tensor& t) {
@@ -316,7 +325,7 @@ std::tuple<Tensor, Tensor> gated_scan(Tensor g, OptTensor h0, OptTensor mask) {
                       mask->sizes(), " on ", mask->device());
     mask = plain(mask->scalar_type() == at::kFloat ? *mask : mask->gt(0));
   }
-  if (tracked(g) || (h0.has_value() && tracked(*h0))) {
+  if (tracked(g, h0, what)) {
     auto out = GatedScan::apply(g, h0, mask);
     return {out[0], out[1]};
   }
@@ -338,7 +347,7 @@ Tensor token_logprob(Tensor logits, Tensor y, OptTensor mask) {
   check_rows(logits, y, what);
   OptTensor w;
   if (mask.has_value()) w = per_token(*mask, logits, what, "mask");
-  if (tracked(logits)) return TokenLogprob::apply(logits, y, w);
+  if (tracked(logits, what)) return TokenLogprob::apply(logits, y, w);
   return token_logprob_fwd(logits, y, w)[0];
 }
 
@@ -361,7 +370,7 @@ std::tuple<Tensor, Tensor> policy_loss(Tensor logits, Tensor y, Tensor mask,
                     ", got ", advantage.sizes(), " on ", advantage.device());
   if (advantage.scalar_type() != at::kFloat || advantage.requires_grad())
     advantage = advantage.detach().to(at::kFloat);
-  if (tracked(logits)) {
+  if (tracked(logits, what)) {
     auto out =
         PolicyLoss::apply(logits, y, w, old, advantage, ref, lo, hi, beta);
     return {out[0], out[1]};
@@ -378,7 +387,7 @@ std::tuple<Tensor, Tensor> preference_loss(Tensor logits, Tensor y, Tensor mask,
   check_rows(logits, y, what);
   Tensor w = per_token(mask, logits, what, "mask");
   Tensor ref = per_token(ref_logp, logits, what, "ref_logp");
-  if (tracked(logits)) {
+  if (tracked(logits, what)) {
     auto out = PreferenceLoss::apply(logits, y, w, ref, beta, eps);
     return {out[0], out[1]};
   }
@@ -403,7 +412,7 @@ Tensor counter_dropout(Tensor x, OptTensor residual, double p, OptTensor rng,
                       "counter_dropout: residual must have x's shape, type and "
                       "device, got ",
                       residual->sizes(), " ", residual->scalar_type());
-  if (tracked(x) || (residual.has_value() && tracked(*residual)))
+  if (tracked(x, residual, "counter_dropout"))
     return CounterDropout::apply(x, residual, p, rng, seed, step, stream);
   return drop(x, residual, order_of(x), p, rng, seed, step, stream, false)[0];
 }
