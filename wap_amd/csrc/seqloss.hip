@@ -5,7 +5,8 @@
 //   d loss / d x_k = c (1[k = y] - exp(x_k - m) / S),  c = d loss / d logp
 //
 // A row of weight 0 is not read: its logp is 0 and its gradient row is zeros.
-// A token outside [0, K) in a row that counts makes its logp NaN.
+// A token outside [0, K) in a row that counts makes its logp NaN, and with it
+// the row's gradient, unless c is 0: nothing depends on the row then.
 // What follows the sums of a row (log, ratio, comparison with the clip's
 // borders, sums over tokens) is in 64 bits: it is one thread's work a row, and
 // an error of 1e-7 there could move a token across a border.
@@ -458,10 +459,13 @@ __device__ __forceinline__ void grad_row(const T* logits, const Rows& r,
   const float w = weight(r, row);
   T* d = dlogits + row * r.K;
   if (w == 0.f) return zero_span<COLD>(d, r.K, begin, end, lane, step);
-  const float c = factor(f, r, row, w);
+  const long y = r.y[row];
+  float c = factor(f, r, row, w);
+  // of a token that is none: what depends on its NaN is NaN
+  if (c != 0.f && (y < 0 || y >= r.K)) c = NAN;
   const float2 q = stats[row];
-  grad_span<COLD>(logits + row_at(r, row), d, r.K, begin, end, lane, step,
-                  r.y[row], q.x, -c / q.y, c);
+  grad_span<COLD>(logits + row_at(r, row), d, r.K, begin, end, lane, step, y,
+                  q.x, -c / q.y, c);
 }
 
 // Gradient of rows with known statistics: `lanes` threads and a part of the

@@ -11,7 +11,9 @@ past teacher forcing.
 Conventions are those of ``models.masked_ce``: logits [B,T,K], tokens y [B,T],
 weights mask [B,T], loss = sum(mask * l) / max(sum(mask), 1).  A token of
 weight 0 is not looked at (its logits may hold anything) and gets a zero
-gradient.  A token outside [0, K) that counts makes the result NaN.
+gradient.  A token outside [0, K) that counts makes the result NaN, and its
+row's gradient too, unless the upstream gradient of its log-probability is 0
+(whoever replaced the NaN depends on nothing there).
 
 The exponentials of a row are f32; what follows their sum (logarithm, ratio,
 the comparison with the clip's borders, sums over tokens) is f64, since an
@@ -40,7 +42,8 @@ def _live(w: Optional[Tensor], y: Tensor) -> Tensor:
 
 
 def _rows(logits: Tensor, y: Tensor, w: Optional[Tensor]):
-    """(logp f64, exponentials, their sum f64, safe token, live) — eager."""
+    """(logp f64, exponentials, their sum f64, safe token, live, inside) —
+    eager."""
     live = _live(w, y)
     k = logits.shape[-1]
     inside = (y >= 0) & (y < k)
@@ -52,12 +55,14 @@ def _rows(logits: Tensor, y: Tensor, w: Optional[Tensor]):
     logp = (x.gather(-1, at.unsqueeze(-1)).double() - top.double()
             - torch.log(total)).squeeze(-1)
     logp = torch.where(inside, logp, float("nan"))
-    return torch.where(live, logp, 0.0), e, total, at, live
+    return torch.where(live, logp, 0.0), e, total, at, live, inside
 
 
 def _rows_grad(logits: Tensor, e: Tensor, total: Tensor, at: Tensor,
-               live: Tensor, coef: Tensor) -> Tensor:
-    """coef * (1[k = y] - p), zeros in rows that do not count — eager."""
+               live: Tensor, inside: Tensor, coef: Tensor) -> Tensor:
+    """coef * (1[k = y] - p), zeros in rows that do not count, NaN for a token
+    outside [0, K) that anything depends on — eager."""
+    coef = torch.where(inside | (coef == 0), coef, float("nan"))
     d = e * (-coef.unsqueeze(-1) / total).to(e.dtype)
     d.scatter_add_(-1, at.unsqueeze(-1), coef.unsqueeze(-1).to(e.dtype))
     return torch.where(live.unsqueeze(-1), d, 0.0).to(logits.dtype)
@@ -75,8 +80,8 @@ class _TokenLogprob(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dlogp: Tensor):
         logits, y, w = ctx.saved_tensors
-        _, e, total, at, live = _rows(logits, y, w)
-        return _rows_grad(logits, e, total, at, live, dlogp.double()), None, None
+        _, *rows = _rows(logits, y, w)
+        return _rows_grad(logits, *rows, dlogp.double()), None, None
 
 
 def _policy_terms(logp, old, adv, ref, lo, hi, beta):
@@ -101,7 +106,7 @@ class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, y, w, old, adv, ref, lo, hi, beta):
         ctx.set_materialize_grads(False)
-        logp, e, total, at, live = _rows(logits, y, w)
+        logp, _, _, _, live, _ = _rows(logits, y, w)
         l, slope = _policy_terms(logp, old, adv, ref, lo, hi, beta)
         share = w.double() / w.double().sum().clamp_min(1.0)
         loss = torch.where(live, share * l, 0.0).sum().to(_up(logits).dtype)
@@ -118,15 +123,15 @@ class _PolicyLoss(torch.autograd.Function):
         if up is None:
             return None, *none
         logits, y, w, coef = ctx.saved_tensors
-        _, e, total, at, live = _rows(logits, y, w)
-        return _rows_grad(logits, e, total, at, live, coef * up.double()), *none
+        _, *rows = _rows(logits, y, w)
+        return _rows_grad(logits, *rows, coef * up.double()), *none
 
 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, y, w, ref, beta, eps):
         ctx.set_materialize_grads(False)
-        logp, e, total, at, live = _rows(logits, y, w)
+        logp, _, _, _, live, _ = _rows(logits, y, w)
         gain = torch.where(live, w.double() * (logp - ref.double()), 0.0).sum(1)
         pairs = logits.shape[0] // 2
         m = beta * (gain[:pairs] - gain[pairs:])
@@ -154,9 +159,9 @@ class _PreferenceLoss(torch.autograd.Function):
         if up is None:
             return None, *none
         logits, y, w, seq = ctx.saved_tensors
-        _, e, total, at, live = _rows(logits, y, w)
+        _, *rows = _rows(logits, y, w)
         coef = w.double() * seq.unsqueeze(1) * up.double()
-        return _rows_grad(logits, e, total, at, live, coef), *none
+        return _rows_grad(logits, *rows, coef), *none
 
 
 def _check(logits: Tensor, y: Tensor, mask: Optional[Tensor], what: str):
