@@ -59,17 +59,17 @@ __device__ __forceinline__ float exp_of(float x) {
 }
 
 // z = 1 / (1 + e), 1 - z = e z with e = exp(-gz), cut at 2^126 so that the
-// product stays finite.  tanh x = 1 - 2 / (1 + exp(2 x)), absolute error
-// 1.2e-7; near zero, where that is not enough, the odd series: to x^5 below 0.1
-// (the next term is 6e-8 of the value there), for f32 gates to x^9 below 0.3
-// (5e-8).
+// product stays finite; where it is cut z is 0.  tanh x = 1 - 2 / (1 + exp(2
+// x)), absolute error 1.2e-7; near zero, where that is not enough, the odd
+// series: to x^5 below 0.1 (the next term is 6e-8 of the value there), for f32
+// gates to x^9 below 0.3 (5e-8).
 template <typename T>
 __device__ __forceinline__ Gates gates(float gz, float gn) {
   const float e = exp_of<T, -1, true>(gz);
   Gates r;
   const float z = __builtin_amdgcn_rcpf(1.f + e);
   r.zc = e * z;
-  r.z = z - 0x1p-126f;  // nothing but where e was cut: 0
+  r.z = e >= 0x1p126f ? 0.f : z;  // NaN stays
   const float f = exp_of<T, 2, false>(gn);
   const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + f), 1.f);
   const float q = gn * gn;
