@@ -35,19 +35,25 @@ def _limit(p: float) -> int:
     return math.floor(p * 65536 + 0.5)
 
 
-def _draws(n: int, rng: Tensor, stream: int) -> Tensor:
-    """The n 16-bit draws in storage order (int64 arithmetic, wrapping)."""
-    group = torch.arange((n + 7) // 8, device=rng.device)
-    c0, c1 = group & _LOW, (stream << 8) | (group >> 32)
-    c2 = (rng[1] & _LOW).expand_as(c0)
-    c3 = ((rng[1] >> 32) & _LOW).expand_as(c0)
-    k0, k1 = rng[0] & _LOW, (rng[0] >> 32) & _LOW
+def _words(c0: Tensor, c1: Tensor, c2: Tensor, c3: Tensor, k0: Tensor,
+           k1: Tensor) -> Tensor:
+    """The generator's four words [..., 4] of a counter and a key (32 bits
+    each, in int64 arithmetic, wrapping)."""
     for _ in range(7):
         p, q = c0 * 0xD2511F53, c2 * 0xCD9E8D57
         c0, c1, c2, c3 = (((q >> 32) & _LOW) ^ c1 ^ k0, q & _LOW,
                           ((p >> 32) & _LOW) ^ c3 ^ k1, p & _LOW)
         k0, k1 = (k0 + 0x9E3779B9) & _LOW, (k1 + 0xBB67AE85) & _LOW
-    words = torch.stack([c0, c1, c2, c3], dim=-1)
+    return torch.stack([c0, c1, c2, c3], dim=-1)
+
+
+def _draws(n: int, rng: Tensor, stream: int) -> Tensor:
+    """The n 16-bit draws in storage order."""
+    group = torch.arange((n + 7) // 8, device=rng.device)
+    c0, c1 = group & _LOW, (stream << 8) | (group >> 32)
+    c2 = (rng[1] & _LOW).expand_as(c0)
+    c3 = ((rng[1] >> 32) & _LOW).expand_as(c0)
+    words = _words(c0, c1, c2, c3, rng[0] & _LOW, (rng[0] >> 32) & _LOW)
     return torch.stack([words & 0xFFFF, words >> 16], dim=-1).view(-1)[:n]
 
 
