@@ -7,9 +7,9 @@
 // A row of weight 0 is not read: its logp is 0 and its gradient row is zeros.
 // A token outside [0, K) in a row that counts makes its logp NaN, and with it
 // the row's gradient, unless c is 0: nothing depends on the row then.
-// What follows the sums of a row (log, ratio, comparison with the clip's
-// borders, sums over tokens) is in 64 bits: it is one thread's work a row, and
-// an error of 1e-7 there could move a token across a border.
+// The sums of a row and what follows them (log, ratio, comparison with the
+// clip's borders, sums over tokens) are in 64 bits: an error of 1e-7 there could
+// move a token across a border, and a gain adds up those of hundreds of tokens.
 #include <hip/hip_runtime.h>
 
 #include "opcommon.h"
@@ -83,34 +83,56 @@ __device__ __forceinline__ float exp_from(float x, float m) {
   return __builtin_amdgcn_exp2f(log2_from(x, m));
 }
 
-// Exponentials e = 2^u of a row, added up.  What LOG2E lacks makes every e too
-// large by u LOST ln 2, always to the same side (5e-8 of the sum, and a
-// gain adds up the logarithms of hundreds): the sum of e u takes it back.
+// Exponentials of a row, added up.  The sum is 64-bit: a row's largest
+// exponential is 1, and an f32 sum beside it would round every other one to
+// 2^-24, which a gain over hundreds of tokens adds up.  What e = exp2(u) lacks
+// goes into `t`, to first order, and is a millionth of the sum: f32.
+// - f32 logits: u's own rounding and LOG2E's, from two products more.
+// - 16-bit logits, whose differences have few bits: LOG2E's alone, which makes
+//   every e too large by u LOST ln 2 (5e-8 of the sum).
+template <typename T>
 struct Sum {
-  float s, t;
+  static constexpr bool FINE = sizeof(T) == 4;
+  double s = 0.0;
+  float t = 0.f;
 
-  __device__ __forceinline__ void add(float x, float m) {
-    // 2^-150 is nothing beside the maximum's 1, and e u stays finite
-    const float u = __builtin_elementwise_maximum(log2_from(x, m), -150.f);
+  // e, and its share of t
+  __device__ __forceinline__ float take(float x, float m) {
+    // 2^-150 is nothing beside the maximum's 1, and what it is multiplied with
+    // stays finite
+    const float d = __builtin_elementwise_maximum(x - m, -104.f);
+    const float u = d * LOG2E;
     const float e = __builtin_amdgcn_exp2f(u);
-    s += e;
-    t = fmaf(e, u, t);
+    if constexpr (FINE)
+      t = fmaf(e, fmaf(d, (float)(LOST * LOG2E), fmaf(d, LOG2E, -u)), t);
+    else
+      t = fmaf(e, u, t);
+    return e;
+  }
+  __device__ __forceinline__ void add(float x, float m) {
+    s += (double)take(x, m);
   }
   __device__ __forceinline__ void add(const Sum& o) {
     s += o.s;
     t += o.t;
   }
-  // to another maximum, m <= top
-  __device__ __forceinline__ void move(float m, float top) {
-    const float u = __builtin_elementwise_maximum(log2_from(m, top), -150.f);
-    const float e = __builtin_amdgcn_exp2f(u);
-    t = e * fmaf(u, s, t);
-    s *= e;
+  // to another maximum
+  __device__ __forceinline__ void scale(double f) {
+    s *= f;
+    t *= (float)f;
   }
   __device__ __forceinline__ double value() const {
-    return (double)s + (double)t * (LOST * 0.693147180559945309417);
+    constexpr double ln2 = 0.693147180559945309417;
+    return s + (double)t * (FINE ? ln2 : LOST * ln2);
   }
 };
+
+// The hardware's exp2 is too small by this share on average (all fractions
+// alike, arguments in [-30, 0]: 3.4e-9 in each octave below -1/2), exp2(0) is
+// exact: a sum `v` of which `exact` is the largest's, with that put right.
+__device__ __forceinline__ double with_mean(double v, double exact) {
+  return v + 3.4e-9 * (v - exact);
+}
 
 // Over the workgroup, on every thread; `red`: one value a wave.
 // The sum of the threads' parts is in 64 bits, for the logarithm.
@@ -260,8 +282,9 @@ __device__ __forceinline__ void zero_span(T* d, int K, int begin, int end,
 // NT threads a row.  E > 0: the row waits in registers, E 16-byte vectors a
 // thread, packed as they came.  E = 0: rows too long for that are read once
 // for the sums (a running maximum and sum a thread) and again for the
-// gradient.  Bound by memory: about 20 instruction slots an element of bf16 are
-// half of what reading and writing it takes.
+// gradient.  Bound by memory: the vector work stays behind it, that of the
+// 64-bit sums too (8192 x 32768 bf16 policy 189 us, 4096 x 131072 bf16 logprob
+// 133, 4206 x 50001 f32 preference 413; with f32 sums 189, 132, 413).
 template <typename T, int NT, int E, bool POLICY, bool COLD>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
     const T* __restrict__ logits, Rows r, Policy p,
@@ -303,7 +326,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
   constexpr int HELD = E > 0 ? E : 1;
   vec raw[HELD];
   float m = tail;
-  Sum sum{0.f, 0.f};
+  double mine;  // this thread's part of the sum
   if constexpr (E > 0) {
 #pragma unroll
     for (int e = 0; e < E; ++e)
@@ -333,23 +356,24 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
         for (int i = 0; i < V; ++i) m = fmaxf(m, (float)raw[e][i]);
       }
     m = group_max<NT>(m, red_max);
-    Sum part[4] = {};  // several chains of additions
+    Sum<T> part[2];  // two chains of additions
     if (tid < rest) part[0].add(tail, m);
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (e * NT + tid < whole) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) part[i & 3].add((float)raw[e][i], m);
+        for (int i = 0; i < V; ++i) part[i & 1].add((float)raw[e][i], m);
       }
     part[0].add(part[1]);
-    part[2].add(part[3]);
-    sum = part[0];
-    sum.add(part[2]);
+    mine = part[0].value();
   } else {
-    // a thread's own maximum and sum; the maximum never holds a NaN, the sum
-    // keeps one
-    m = fmaxf(m, -INFINITY);
-    if (tid < rest) sum.s = tail == tail ? 1.f : NAN;
+    // A thread's own maximum, and its sum from an earlier one, `m`: the sum
+    // moves only where exponentials would pass e^8.  Neither ever holds a NaN;
+    // the sum keeps one.
+    float top = fmaxf(m, -INFINITY);
+    m = top;
+    Sum<T> part[2];
+    if (tid < rest) part[0].s = tail != tail ? (double)NAN : tail > -INFINITY ? 1.0 : 0.0;
     constexpr int U = 4;
     for (int i0 = tid; i0 < whole; i0 += U * NT) {
       vec q[U];
@@ -357,38 +381,49 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rows_kernel(
       for (int u = 0; u < U; ++u)
         if (i0 + u * NT < whole)
           q[u] = *reinterpret_cast<const vec*>(x + cut.vec_at(i0 + u * NT));
-      float top = m;
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (i0 + u * NT < whole) {
 #pragma unroll
           for (int i = 0; i < V; ++i) top = fmaxf(top, (float)q[u][i]);
         }
-      // (all minus infinity so far: nothing to move)
-      if (top > m && sum.s != 0.f) sum.move(m, top);
-      m = top;
+      if (top > m + 8.f) {
+        // (all minus infinity so far: nothing to move)
+        if (m > -INFINITY) {
+          part[0].add(part[1]);
+          part[0].scale(exp((double)m - (double)top));
+          part[1] = Sum<T>();
+        }
+        m = top;
+      }
       const float at = m == -INFINITY ? 0.f : m;
-      Sum part[4] = {};
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (i0 + u * NT < whole) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) part[i & 3].add((float)q[u][i], at);
+          for (int i = 0; i < V; ++i) part[i & 1].add((float)q[u][i], at);
         }
-      part[0].add(part[1]);
-      part[2].add(part[3]);
-      sum.add(part[0]);
-      sum.add(part[2]);
     }
-    const float all = group_max<NT>(m, red_max);
-    if (m == -INFINITY && all > m) {
-      if (sum.s == sum.s) sum = Sum{0.f, 0.f};
-    } else {
-      sum.move(m, all);
+    part[0].add(part[1]);
+    const float all = group_max<NT>(top, red_max);
+    mine = 0.0;
+    if (m > -INFINITY) {
+      Sum<T> one;
+      one.add(top, m);
+      const double v = part[0].value(), largest = one.value();
+      mine = with_mean(v, largest);
+      // the row's largest is 1 exactly, not what exp2 made of it
+      const bool holds = top == all;
+      if (holds) mine -= largest;
+      mine *= exp((double)m - (double)all);
+      if (holds) mine += 1.0;
+    } else if (part[0].s != part[0].s) {
+      mine = NAN;
     }
     m = all;
   }
-  const double total_exp = group_sum<NT>(sum.value(), red_sum);
+  double total_exp = group_sum<NT>(mine, red_sum);
+  if (E > 0) total_exp = with_mean(total_exp, 1.0);
   const float s = (float)total_exp;
   float c = 0.f;
   if (NT == 64 || threadIdx.x < 64) {

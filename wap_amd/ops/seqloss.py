@@ -15,9 +15,9 @@ gradient.  A token outside [0, K) that counts makes the result NaN, and its
 row's gradient too, unless the upstream gradient of its log-probability is 0
 (whoever replaced the NaN depends on nothing there).
 
-The exponentials of a row are f32; what follows their sum (logarithm, ratio,
-the comparison with the clip's borders, sums over tokens) is f64, since an
-error of 1e-7 there can move a token across a border and a gain is a small
+The exponentials of a row are f32; their sum and what follows it (logarithm,
+ratio, the comparison with the clip's borders, sums over tokens) are f64, since
+an error of 1e-7 there can move a token across a border and a gain is a small
 difference of long sums.
 """
 
