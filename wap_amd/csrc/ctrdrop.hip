@@ -44,9 +44,9 @@ __device__ __forceinline__ Draws draws(
 // One thread per group of eight elements, 16 or 2 x 16 bytes a load.  Bound by
 // memory: a draw of eight is 7 rounds of two 32x32->64-bit products and four
 // xors, about 12 slots an element, half of what reading and writing 16-bit
-// values takes.  16384 x 4096 fp16 on an MI355X: 40 us (6.7 TB/s), with a
-// residual 70 us (5.7 TB/s), where a copy reaches 5.1; two or four groups a
-// thread are slower (43, 47 us): the chip is full of waves as it is.
+// values takes.  16384 x 4096 fp16 on an MI355X, a call among others: 40 us (6.7
+// TB/s), with a residual 69 us (5.8 TB/s), where a copy reaches 5.1; two or four
+// groups a thread are slower (43, 47 us): the chip is full of waves as it is.
 constexpr int THREADS = 256;
 
 template <typename T, bool RES>

@@ -307,9 +307,9 @@ __device__ __forceinline__ Global<V> lane_at(T* row, uint32_t bytes) {
 
 // COLD: past the caches, where a pass moves more than the 256 MB of the last
 // one, so that none of it would be there for the next reader (8 x 8192 x 2048
-// bf16: forward 206 us, 217 without, backward 285, 307).  Not where channel
+// bf16: forward 172 us, 178 without, backward 302, 312).  Not where channel
 // blocks share cache lines: the caches put those together (4 x 8000 x 1001
-// f32: forward 92.5 us, with cold stores 99.5, with cold loads too 108).
+// f32: forward 92 us, with cold stores 99, with cold loads too 108).
 template <bool COLD, typename V, typename T>
 __device__ __forceinline__ void put(T* row, uint32_t bytes, const V& v) {
   if constexpr (COLD)
@@ -679,18 +679,19 @@ struct Shape {
 };
 
 // How a pass is cut, by the number of 64-channel blocks and the length (us on
-// an MI355X; "2,8,16": two channels a lane, 8 waves of 16 steps).
+// an MI355X, a call among others; "2,8,16": two channels a lane, 8 waves of 16
+// steps).
 // - Up to 256 steps one tile holds the sequence, and nothing is chained: 16 x
-//   200 x 256 bf16 forward 8.2 in one tile of 1,16,16, 10.7 in two of 1,8,16.
+//   200 x 256 bf16 forward 7.9 in one tile of 1,16,16, 10.4 in two of 1,8,16.
 // - Few blocks: time is the only axis to spread over, and a round trip of the
-//   chain should step far: 1 x 40000 x 128 bf16 forward 28.5 with tiles of 256
-//   steps, 55.6 with 128; from 5 blocks on 128 (2 x 20000 x 512: 48.7, 40.8).
+//   chain should step far: 1 x 40000 x 128 bf16 forward 27 with tiles of 256
+//   steps, 55 with 128; from 5 blocks on 128 (2 x 20000 x 512: 51, 45).
 // - Two channels a lane where that leaves enough workgroups, from 64 blocks on
-//   (short sequences, all latency, from 128): 32 x 4096 x 256 bf16 forward
-//   53.8, with one 65.5; 4 x 8192 x 1500: 87, 135; 8 x 4096 x 256: 21.1, 21.7;
-//   16 x 200 x 256: 10.2, 8.2.  The backward pass then holds 8 steps a wave, to
-//   stay under 128 registers: 8 x 8192 x 2048 283, with 16 steps of one channel
-//   340.
+//   (short sequences, all latency, from 128): 32 x 4096 x 256 bf16 forward 53,
+//   with one 65; 4 x 8192 x 1500: 79, 119; with 32 blocks, 8 x 4096 x 256, 20,
+//   21; 16 x 200 x 256: 10.2, 7.9.  The backward pass then holds 8 steps a wave,
+//   to stay under 128 registers: 8 x 8192 x 2048 302, with 16 steps of one
+//   channel 320.
 Shape shape_of(const torch::Tensor& g, bool backward) {
   const long L = g.size(1), D = g.size(2) / 2;
   const long blocks = g.size(0) * ((D + 63) / 64);
